@@ -26,7 +26,8 @@ import re
 HERE = pathlib.Path(__file__).resolve().parent
 LIB_PATH = HERE / "libqgemv.so"
 HEADER_PATH = HERE.parent / "include" / "qgemv.h"
-HEADERS = (HEADER_PATH, HERE.parent / "include" / "qgmodel.h", HERE.parent / "include" / "qggguf.h")
+HEADERS = (HEADER_PATH, HERE.parent / "include" / "qgmodel.h", HERE.parent / "include" / "qggguf.h",
+           HERE.parent / "include" / "qgops.h")
 
 # GGML type ids, src/gguf.rs:43-59
 F32, F16, Q4_0, Q4_1, Q5_0, Q5_1, Q8_0, Q8_1, Q2_K, Q3_K, Q4_K, Q5_K, Q6_K = (
@@ -134,7 +135,22 @@ _SIGS = {
     "qg_model_sample_greedy": (ctypes.c_int, [_P, _P, _SZ, ctypes.c_float, _SZ, ctypes.POINTER(_U32)]),
     "qg_model_generate": (ctypes.c_int, [_P, _P, _SZ, _SZ, ctypes.c_float, _SZ, _P,
                                          ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]),
+    # include/qgops.h
+    "qg_kv8_create": (ctypes.c_int, [_P, _SZ, _SZ, _SZ, _SZ, ctypes.POINTER(_P)]),
+    "qg_kv8_free": (ctypes.c_int, [_P, _P]),
+    "qg_kv8_info": (ctypes.c_int, [_P] + [ctypes.POINTER(_SZ)] * 5),
+    "qg_kv8_write_dev": (ctypes.c_int, [_P, _P, _P, _P, _P, _P]),
+    "qg_kv8_read_dev": (ctypes.c_int, [_P, _P, _SZ, _SZ, _SZ, _SZ, _P, _P, _P]),
+    "qg_kv8_attention_dev": (ctypes.c_int, [_P, _P, _P, _SZ, _P, ctypes.c_float, _SZ, _P, _P, _SZ, _P]),
+    "qg_kv8_attention_work": (ctypes.c_int, [_P, _P, _SZ, _SZ, ctypes.POINTER(_SZ)]),
+    "qg_logprobs_dev": (ctypes.c_int, [_P, _P, _U32, _SZ, _SZ, _SZ, _P, _SZ, _P, _P, _SZ, _P, _P, _P, _SZ, _P]),
+    "qg_logprobs_work": (ctypes.c_int, [_P, _SZ, _SZ, _SZ, ctypes.POINTER(_SZ)]),
 }
+
+# include/qgops.h
+KV8_BLOCK = 32
+LOGPROBS_MAX_TOP = 64
+TOKEN_NONE = 0xFFFFFFFF
 
 # include/qgmodel.h slots (names of the GGUF tensors, src/model.rs:197-298)
 M_TOKEN_EMBD, M_LM_HEAD, M_WQ, M_WK, M_WV, M_WO, M_GATE, M_UP, M_DOWN = range(9)
@@ -146,6 +162,17 @@ class ModelConfig(ctypes.Structure):
     _fields_ = [(n, ctypes.c_uint32) for n in ("embed_dim", "n_layers", "n_heads", "n_kv_heads",
                                                  "hidden_dim", "vocab_size", "max_seq_len")] + \
                [("rope_base", ctypes.c_float), ("norm_eps", ctypes.c_float)]
+
+
+class Rows(ctypes.Structure):
+    """qg_rows: rows [row][head][head_dim] on the device (include/qgops.h)."""
+    _fields_ = [("data", _P), ("type", _U32), ("ld_row", _SZ), ("ld_head", _SZ)]
+
+
+class Batch(ctypes.Structure):
+    """qg_batch: the rows of every sequence of a call (include/qgops.h)."""
+    _fields_ = [("n_rows", _SZ), ("d_starts", _P), ("d_lens", _P)]
+
 
 _lib = None
 
@@ -332,6 +359,127 @@ class GpuContext:
         """Test hook: after `skip` more allocations, the next n allocations of
         this context report out-of-memory (qg_test_fail_allocations)."""
         self.check(self.lib.qg_test_fail_allocations(self.h, int(skip), int(n)), "qg_test_fail_allocations")
+
+
+    def kv8(self, n_seqs: int, n_kv_heads: int, head_dim: int, max_len: int) -> "Kv8Cache":
+        """An 8-bit KV cache of one attention layer (qg_kv8_create)."""
+        h = _P()
+        self.check(self.lib.qg_kv8_create(self.h, n_seqs, n_kv_heads, head_dim, max_len, ctypes.byref(h)),
+                   "qg_kv8_create")
+        return Kv8Cache(self, h, n_seqs, n_kv_heads, head_dim, max_len)
+
+    def logprobs_work(self, n_rows: int, n_cols: int, k: int = 0) -> int:
+        """Bytes of workspace logprobs_dev needs (qg_logprobs_work)."""
+        n = _SZ()
+        self.check(self.lib.qg_logprobs_work(self.h, n_rows, n_cols, k, ctypes.byref(n)), "qg_logprobs_work")
+        return n.value
+
+    def logprobs_dev(self, logits, tokens, logprobs, entropy=None, top_ids=None, top_logprobs=None, work=None,
+                     stream=None):
+        """Log probabilities of tokens [rows, given] (int32, or None) under
+        logits [rows, cols] (float32 or float16), the entropy [rows(, 1)] and
+        the most likely tokens [rows, k] of every row; torch device tensors
+        (qg_logprobs_dev).  work: at least logprobs_work bytes."""
+        rows, cols = logits.shape
+        if logits.stride(1) != 1 and cols > 1:
+            raise QgemvError(7, "logits of a row are not contiguous")
+        given = tokens.shape[1] if tokens is not None else 0
+        k = top_ids.shape[1] if top_ids is not None else 0
+        for t, size, n in ((tokens, 4, rows * given), (logprobs, 4, rows * given), (entropy, 4, rows),
+                           (top_ids, 4, rows * k), (top_logprobs, 4, rows * k)):
+            if t is not None and (t.element_size() != size or t.numel() != n or not t.is_contiguous()):
+                raise QgemvError(7, "an array of logprobs_dev has another shape or type, or is not contiguous")
+        self.check(self.lib.qg_logprobs_dev(self.h, _ptr(logits), _row_type(logits), rows, cols, logits.stride(0),
+                                            _ptr(tokens), given, _ptr(logprobs), _ptr(entropy), k, _ptr(top_ids),
+                                            _ptr(top_logprobs), _ptr(work), _nbytes(work),
+                                            ctypes.c_void_p(stream) if stream else None), "qg_logprobs_dev")
+
+
+def _nbytes(t) -> int:
+    return 0 if t is None else t.numel() * t.element_size()
+
+
+def _row_type(t) -> int:
+    """GGML id of a torch tensor's type (any but float32 and float16: one the library refuses)."""
+    return {"torch.float32": F32, "torch.float16": F16}.get(str(t.dtype), 0xFFFFFFFF)
+
+
+def _rows(t, n_rows: int, heads: int, hd: int, what: str) -> Rows:
+    """qg_rows of a torch tensor [rows, heads, head_dim]."""
+    if tuple(t.shape) != (n_rows, heads, hd) or (hd > 1 and t.stride(2) != 1):
+        raise QgemvError(7, f"{what} is not [{n_rows}, {heads}, {hd}] with contiguous elements")
+    return Rows(t.data_ptr(), _row_type(t), t.stride(0), t.stride(1))
+
+
+class Kv8Cache:
+    """Keys and values of one attention layer in 8 bits (qg_kv8).  Tensors are
+    torch device tensors; lens [n_seqs] and starts [n_seqs + 1] are int32."""
+
+    def __init__(self, ctx: GpuContext, h, n_seqs: int, n_kv_heads: int, head_dim: int, max_len: int):
+        self.ctx, self.h = ctx, h
+        self.n_seqs, self.n_kv_heads, self.head_dim, self.max_len = n_seqs, n_kv_heads, head_dim, max_len
+
+    def free(self):
+        # a closed context has already freed its caches (qg_destroy)
+        if self.h and self.ctx.h:
+            self.ctx.check(self.ctx.lib.qg_kv8_free(self.ctx.h, self.h), "qg_kv8_free")
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+    @property
+    def nbytes(self) -> int:
+        n = _SZ()
+        self.ctx.check(self.ctx.lib.qg_kv8_info(self.h, None, None, None, None, ctypes.byref(n)), "qg_kv8_info")
+        return n.value
+
+    def _batch(self, n_rows: int, lens, starts) -> Batch:
+        for t, n in ((lens, self.n_seqs), (starts, self.n_seqs + 1)):
+            if t is not None and (t.element_size() != 4 or t.numel() != n or not t.is_contiguous()):
+                raise QgemvError(7, "lens or starts: one int32 per sequence, one more of the starts")
+        return Batch(n_rows, _ptr(starts), _ptr(lens))
+
+    def write_dev(self, k, v, lens, starts=None, stream=None):
+        """Cache k and v [rows, n_kv_heads, head_dim]; lens: every sequence's
+        positions with these rows (qg_kv8_write_dev)."""
+        n = k.shape[0]
+        b = self._batch(n, lens, starts)
+        rk, rv = (_rows(t, n, self.n_kv_heads, self.head_dim, w) for t, w in ((k, "k"), (v, "v")))
+        self.ctx.check(self.ctx.lib.qg_kv8_write_dev(self.ctx.h, self.h, ctypes.byref(b), ctypes.byref(rk),
+                                                     ctypes.byref(rv), ctypes.c_void_p(stream) if stream else None),
+                       "qg_kv8_write_dev")
+
+    def read_dev(self, seq: int, n_seqs: int, pos: int, n: int, k=None, v=None, stream=None):
+        """Positions pos .. pos + n of n_seqs sequences from seq on as values
+        [n_seqs * n, n_kv_heads, head_dim] (qg_kv8_read_dev)."""
+        rk, rv = (None if t is None else _rows(t, n_seqs * n, self.n_kv_heads, self.head_dim, w)
+                  for t, w in ((k, "k"), (v, "v")))
+        self.ctx.check(self.ctx.lib.qg_kv8_read_dev(self.ctx.h, self.h, seq, n_seqs, pos, n,
+                                                    None if rk is None else ctypes.byref(rk),
+                                                    None if rv is None else ctypes.byref(rv),
+                                                    ctypes.c_void_p(stream) if stream else None), "qg_kv8_read_dev")
+
+    def attention_work(self, n_rows: int, n_heads: int) -> int:
+        """Bytes of workspace attention_dev needs (qg_kv8_attention_work)."""
+        n = _SZ()
+        self.ctx.check(self.ctx.lib.qg_kv8_attention_work(self.ctx.h, self.h, n_rows, n_heads, ctypes.byref(n)),
+                       "qg_kv8_attention_work")
+        return n.value
+
+    def attention_dev(self, q, out, lens, work=None, starts=None, scale=None, window: int = 0, stream=None):
+        """out = attention of q [rows, n_heads, head_dim] over the cache; scale:
+        1 / sqrt(head_dim) by default (qg_kv8_attention_dev)."""
+        n, heads = q.shape[0], q.shape[1]
+        b = self._batch(n, lens, starts)
+        rq, ro = (_rows(t, n, heads, self.head_dim, w) for t, w in ((q, "q"), (out, "out")))
+        self.ctx.check(self.ctx.lib.qg_kv8_attention_dev(
+            self.ctx.h, self.h, ctypes.byref(b), heads, ctypes.byref(rq),
+            float(self.head_dim ** -0.5 if scale is None else scale), window, ctypes.byref(ro), _ptr(work), _nbytes(work),
+            ctypes.c_void_p(stream) if stream else None), "qg_kv8_attention_dev")
 
 
 class DeviceMatrix:

@@ -14,6 +14,7 @@
 #include "qgemv.h"
 
 struct qg_model;
+struct qg_kv8;
 
 struct qg_mat {
     qg_ctx *ctx;
@@ -61,6 +62,7 @@ struct qg_ctx {
     float *d_static_scratch = nullptr;
     std::set<qg_mat *> mats;
     std::set<qg_model *> models;            // decode-step engines on this context
+    std::set<qg_kv8 *> kv8s;                // 8-bit KV caches (qg_kv8_create)
     // qg_gpu_mat_vec_mul's device copies, keyed by (host address, bytes, type,
     // rows, cols), each with the host bytes it was made from: a fingerprint
     // (sampled windows), or all of them (exact, then fp.size() == the
@@ -109,6 +111,9 @@ struct qg_model;
 // Frees every decode-step engine of the context (qg_model.hip); qg_destroy
 // calls it before freeing the context's matrices.
 void qg_models_free_all(qg_ctx *ctx);
+
+// Frees every cache of qg_kv8_create (qg_kv8.hip); qg_destroy calls it.
+void qg_kv8_free_all(qg_ctx *ctx);
 
 // y = W · (rmsnorm(xa + xb) * nw), sum_out (may be NULL) = xa + xb (xb may be
 // NULL: then xa alone).  The stream kernel does the norm in its prologue when

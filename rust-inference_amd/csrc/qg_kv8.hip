@@ -1,0 +1,597 @@
+// qg_kv8.hip -- the 8-bit KV cache of include/qgops.h: handles, and the
+// kernels that quantise new keys and values into it and read them back.
+#include "qg_kv8.h"
+
+#include <algorithm>
+#include <new>
+
+namespace qg8 {
+namespace {
+
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t v)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+    return v;
+}
+
+// What a call does to one sequence: the positions first .. last of blocks b0 ..
+// bl.  Items are what one workgroup per head takes: item 0 block b0 and, where
+// the last block stays open, that one too (they share the f32 tail); item j >
+// 0 the whole block b0 + j.
+struct Piece {
+    Span s;
+    uint32_t first, end, b0, bl, items;   // positions first .. end
+};
+
+__device__ __forceinline__ Piece piece_of(const Batch &b, uint32_t seq, uint32_t max_len)
+{
+    Piece p;
+    p.s = span_of(b, seq);
+    p.end = min(p.s.len, max_len);
+    p.first = p.s.pos > 0 ? (uint32_t)min(p.s.pos, (int64_t)0xFFFFFFFFll) : 0u;
+    p.b0 = p.bl = p.items = 0;
+    if (p.s.n == 0 || p.first >= p.end) return p;
+    p.b0 = p.first / kBlock;
+    p.bl = (p.end - 1) / kBlock;
+    p.items = p.bl - p.b0 + ((p.bl > p.b0 && p.end % kBlock) ? 0u : 1u);
+    return p;
+}
+
+// The sequence and item of workgroup `want`: the items of the sequences before
+// it are counted 64 sequences at a time, by every wave on its own.  False
+// behind the last item.
+__device__ bool find_item(const Batch &b, uint32_t n_seqs, uint32_t max_len, uint32_t want, uint32_t *seq,
+                          uint32_t *item)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    if (b.lens && !b.starts) {                       // one row each
+        *seq = want;
+        *item = 0;
+        return piece_of(b, want, max_len).items != 0;
+    }
+    uint32_t before = 0;
+    for (uint32_t s0 = 0; s0 < n_seqs; s0 += 64) {
+        uint32_t n = s0 + lane < n_seqs ? piece_of(b, s0 + lane, max_len).items : 0u;
+        const uint32_t own = n;
+#pragma unroll
+        for (uint32_t o = 1; o < 64; o <<= 1) {
+            const uint32_t up = (uint32_t)__shfl_up((int)n, o, 64);
+            if (lane >= o) n += up;
+        }
+        const uint64_t past = __ballot(before + n > want);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            *seq = s0 + (uint32_t)l;
+            *item = want - (before + (uint32_t)__shfl((int)(n - own), l, 64));
+            return true;
+        }
+        before += (uint32_t)__shfl((int)n, 63, 64);
+    }
+    return false;
+}
+
+// x / s to the nearest, ties to even, as a code: the f32 product with 1 / s can
+// be one off next to a half; the remainder x - q s is exact (q s has bits no
+// lower than s / 2's last, and the difference is at most about s / 2), so it
+// decides.
+__device__ __forceinline__ int code_of(float x, float s, float inv)
+{
+    float q = rintf(x * inv);
+    const float r = __builtin_fmaf(-q, s, x), h = 0.5f * s, a = fabsf(r);
+    if (a >= h && s > 0.f) {
+        if (a > h || ((int)q & 1)) q += r > 0.f ? 1.f : -1.f;
+    }
+    return (int)q;
+}
+
+constexpr uint32_t kInf = 0x7F800000u;
+
+// Block `b`'s positions lo .. hi (of 32) from the rows, those before lo from
+// what the cache holds.  One workgroup of 256: thread (t, c): position t =
+// tid / 8, elements 16 (c + 8 i) .. + 16.
+template <int NC>
+__device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint64_t ld_row, uint32_t sh, uint64_t base,
+                            uint32_t b, uint32_t lo, uint32_t hi, int slot, bool held, bool open, bool key,
+                            uint32_t *maxes, uint32_t *red, uint8_t *stage)
+{
+    const uint32_t tid = threadIdx.x, t = tid >> 3, c = tid & 7u, dp = v.dp;
+    uint8_t *codes = v.codes + (base * v.n_blocks + b) * kBlock * dp;
+    float *scale = v.scale + base * v.n_blocks + b;
+    float *tail = v.tail + (base * 2 + (uint32_t)(slot < 0 ? 0 : slot)) * kBlock * dp + t * dp;
+    uint32_t *tail_max = v.tail_max + (base * 2 + (uint32_t)(slot < 0 ? 0 : slot)) * kBlock;
+    float val[NC][16];
+    const bool fresh = t >= lo && t < hi, old = t < lo;
+    const float s_old = *scale;
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < NC; i++) {
+        const uint32_t d = 16u * (c + 8u * i);
+        if (d >= dp) break;
+        if (fresh) {
+            load16(x, row_at + (uint64_t)(t - lo) * ld_row, d, v.hd, val[i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++) val[i][j] = 0.f;
+            if (old && !held)          // a block reopened from its codes
+                for (uint32_t j = 0; j < 16; j++) {
+                    const int8_t q = (int8_t)codes[key ? key_at(t, d + j, dp) : value_at(t, d + j)];
+                    val[i][j] = (float)q * s_old;
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < 16; j++) m = max(m, __float_as_uint(val[i][j]) & 0x7FFFFFFFu);
+    }
+    // a position's largest magnitude, over its eight threads
+    m = max(m, (uint32_t)__shfl_xor((int)m, 1, 64));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 2, 64));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 4, 64));
+    if (old && held) m = tail_max[t];
+    if (c == 0) maxes[t] = m;
+    m = wave_max_u(m);
+    if ((tid & 63u) == 0) red[tid >> 6] = m;
+    __syncthreads();
+    m = max(max(red[0], red[1]), max(red[2], red[3]));
+    float s = __uint_as_float(m) / 127.0f;
+    if (s < 0x1p-126f) s = 0.f;
+    if (m >= kInf) s = __uint_as_float(0x7FC00000u);
+    const float inv = s > 0.f ? 1.0f / s : 0.f;              // NaN: no codes
+    // the block's codes of the positions before lo stand while the scale does
+    const bool again = lo > 0 && (__float_as_uint(s) != __float_as_uint(s_old) || !held);
+    if (again && old && held) {
+#pragma unroll
+        for (int i = 0; i < NC; i++) {
+            const uint32_t d = 16u * (c + 8u * i);
+            if (d >= dp) break;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float4 a = *(const float4 *)(tail + d + 4 * j);
+                val[i][4 * j] = a.x; val[i][4 * j + 1] = a.y; val[i][4 * j + 2] = a.z; val[i][4 * j + 3] = a.w;
+            }
+        }
+    }
+    const bool whole = lo == 0 || again;
+    const bool put = fresh || (old && again);
+#pragma unroll
+    for (int i = 0; i < NC; i++) {
+        const uint32_t d = 16u * (c + 8u * i);
+        if (d >= dp) break;
+        union { uint8_t b[16]; uint4 u; } w;
+        w.u = make_uint4(0, 0, 0, 0);
+        if (s > 0.f && put)
+#pragma unroll
+            for (int j = 0; j < 16; j++) w.b[j] = (uint8_t)(int8_t)code_of(val[i][j], s, inv);
+        if (key) {
+            if (put) *(uint4 *)(codes + key_at(t, d, dp)) = w.u;
+        } else if (whole) {
+            *(uint4 *)(stage + t * (dp + 16) + d) = w.u;
+        } else if (fresh) {
+            for (uint32_t j = 0; j < 16; j++) codes[value_at(t, d + j)] = w.b[j];
+        }
+        // the f32 values of a block that stays open
+        if (open && (fresh || (old && !held)))
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                *(float4 *)(tail + d + 4 * j) = make_float4(val[i][4 * j], val[i][4 * j + 1], val[i][4 * j + 2],
+                                                            val[i][4 * j + 3]);
+    }
+    if (!key && whole) {
+        __syncthreads();
+        // 16 bytes of the layout at a time: two elements at eight positions
+        for (uint32_t u = tid; u < 2 * dp; u += 256) {
+            const uint32_t g = u >> 4 & 3u, d = (u >> 6) * 32u + 2u * (u & 15u);
+            union { uint8_t b[16]; uint4 u; } w;
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) {
+                const uint32_t p = 4u * g + (j & 3u) + (j >> 2) * 16u;
+                const uint16_t two = *(const uint16_t *)(stage + p * (dp + 16) + d);
+                w.b[j] = (uint8_t)two;
+                w.b[8 + j] = (uint8_t)(two >> 8);
+            }
+            *(uint4 *)(codes + u * 16u) = w.u;
+        }
+    }
+    if (tid == 0) *scale = s;
+    if (open && tid < hi && (tid >= lo || !held)) tail_max[tid] = maxes[tid];
+    __syncthreads();
+}
+
+// Grid: (items, heads, keys / values).
+//
+// The scale of a block follows from its largest magnitude, so a new token in a
+// block that is partly there costs its own row and 32 remembered magnitudes
+// while it is not the largest, and the block's f32 rows (kept in one of two
+// slots) when it is.  Two slots, because a call that ends one block and opens
+// another must leave the values of the first: the same call may come again.
+template <int NC> __global__ void __launch_bounds__(256) write_k(View v, Batch b, Rows k, Rows val)
+{
+    __shared__ uint32_t maxes[kBlock], red[4];
+    __shared__ __attribute__((aligned(16))) uint8_t stage[kBlock * (128 * NC + 16)];
+    uint32_t seq, item;
+    if (!find_item(b, v.n_seqs, v.max_len, blockIdx.x, &seq, &item)) return;
+    const bool key = blockIdx.z == 0;
+    const Rows &x = key ? k : val;
+    const Piece p = piece_of(b, seq, v.max_len);
+    const uint32_t head = blockIdx.y, sh = seq * v.n_heads + head;
+    const uint64_t base = (uint64_t)blockIdx.z * v.n_seqs * v.n_heads + sh;
+    // element of the row that holds position pos
+    auto row_at = [&](uint32_t pos) {
+        return (uint64_t)(p.s.row + (uint32_t)((int64_t)pos - p.s.pos)) * x.ld_row + head * x.ld_head;
+    };
+    if (item) {
+        const uint32_t blk = p.b0 + item;
+        write_block<NC>(v, x, row_at(blk * kBlock), x.ld_row, sh, base, blk, 0, kBlock, -1, false, false, key, maxes, red, stage);
+        return;
+    }
+    int32_t *at = v.tail_at + base * 4;
+    int32_t tag[2] = {at[0], at[1]}, fill[2] = {at[2], at[3]};
+    __syncthreads();                                          // read by all before thread 0 writes
+    const uint32_t lo = p.first % kBlock, hi = p.bl == p.b0 ? p.end - p.b0 * kBlock : kBlock;
+    // what is held of this block from lo on, or of later ones, is written anew
+    for (int i = 0; i < 2; i++) {
+        if (tag[i] == (int32_t)p.b0) fill[i] = min(fill[i], (int32_t)lo);
+        if (tag[i] > (int32_t)p.b0 || (tag[i] == (int32_t)p.b0 && fill[i] == 0)) tag[i] = -1;
+    }
+    int slot = tag[0] == (int32_t)p.b0 ? 0 : tag[1] == (int32_t)p.b0 ? 1 : -1;
+    bool held = slot >= 0 && fill[slot] >= (int32_t)lo;
+    if (slot >= 0 && !held) { tag[slot] = -1; }
+    const bool open = hi < kBlock;
+    if (slot < 0 || !held) {
+        slot = tag[0] <= tag[1] ? 0 : 1;                      // the older one gives way
+        held = false;
+    }
+    if (open) {
+        tag[slot] = (int32_t)p.b0;
+        fill[slot] = (int32_t)hi;
+    }
+    write_block<NC>(v, x, row_at(p.first), x.ld_row, sh, base, p.b0, lo, hi, slot, held, open, key, maxes, red, stage);
+    if (p.bl > p.b0 && p.end % kBlock) {
+        const int other = held ? 1 - slot : tag[0] <= tag[1] ? 0 : 1;
+        tag[other] = (int32_t)p.bl;
+        fill[other] = (int32_t)(p.end % kBlock);
+        write_block<NC>(v, x, row_at(p.bl * kBlock), x.ld_row, sh, base, p.bl, 0, p.end % kBlock, other, false, true, key, maxes, red,
+                        stage);
+    }
+    if (threadIdx.x == 0) {
+        at[0] = tag[0];
+        at[1] = tag[1];
+        at[2] = fill[0];
+        at[3] = fill[1];
+    }
+}
+
+// Grid: (blocks, heads * keys / values, sequences); 256 threads.
+__global__ void __launch_bounds__(256) read_k(View v, uint32_t seq0, uint32_t pos, uint32_t n, Rows k, Rows val)
+{
+    const uint32_t blk = pos / kBlock + blockIdx.x, head = blockIdx.y % v.n_heads;
+    const bool key = k.p && blockIdx.y < v.n_heads;
+    const Rows &x = key ? k : val;
+    const uint32_t seq = seq0 + blockIdx.z, dp = v.dp;
+    const uint64_t base = (uint64_t)(key ? 0 : 1) * v.n_seqs * v.n_heads + (uint64_t)seq * v.n_heads + head;
+    const uint8_t *codes = v.codes + (base * v.n_blocks + blk) * kBlock * dp;
+    const float s = v.scale[base * v.n_blocks + blk];
+    const uint64_t out = (uint64_t)blockIdx.z * n, p0 = (uint64_t)blk * kBlock;
+    auto at = [&](uint32_t t, uint32_t d) {
+        return (out + (p0 + t - pos)) * x.ld_row + head * x.ld_head + d;
+    };
+    for (uint32_t u = threadIdx.x; u < 2 * dp; u += 256) {
+        union { int8_t b[16]; uint4 u; } w;
+        w.u = *(const uint4 *)(codes + u * 16u);
+        if (key) {
+            // unit u of 16 bytes: position and 16 elements
+            const uint32_t t = (u >> 6) / (dp >> 6) * 16u + (u & 15u), d = (u >> 6) % (dp >> 6) * 64u + (u >> 4 & 3u) * 16u;
+            if (p0 + t < pos || p0 + t >= (uint64_t)pos + n) continue;
+            if (x.vec && d < v.hd) {
+                if (x.f16) {
+                    union { _Float16 h[16]; uint4 u[2]; } y;
+#pragma unroll
+                    for (int j = 0; j < 16; j++) y.h[j] = (_Float16)((float)w.b[j] * s);
+                    uint4 *o = (uint4 *)((_Float16 *)x.p + at(t, d));
+                    o[0] = y.u[0];
+                    o[1] = y.u[1];
+                } else {
+                    float4 *o = (float4 *)((float *)x.p + at(t, d));
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        o[j] = make_float4((float)w.b[4 * j] * s, (float)w.b[4 * j + 1] * s, (float)w.b[4 * j + 2] * s,
+                                           (float)w.b[4 * j + 3] * s);
+                }
+            } else {
+                for (uint32_t j = 0; j < 16; j++)
+                    if (d + j < v.hd) store1(x, at(t, d + j), (float)w.b[j] * s);
+            }
+        } else {
+            const uint32_t g = u >> 4 & 3u, d = (u >> 6) * 32u + 2u * (u & 15u);
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) {
+                const uint32_t t = 4u * g + (j & 3u) + (j >> 2) * 16u;
+                if (p0 + t < pos || p0 + t >= (uint64_t)pos + n) continue;
+                if (d < v.hd) store1(x, at(t, d), (float)w.b[j] * s);
+                if (d + 1 < v.hd) store1(x, at(t, d + 1), (float)w.b[8 + j] * s);
+            }
+        }
+    }
+}
+
+int launched()
+{
+    return hipPeekAtLastError() == hipSuccess ? 0 : -1;
+}
+
+}  // namespace
+
+int launch_write(const View &v, const Batch &b, const Rows &k, const Rows &x, hipStream_t st)
+{
+    if (b.n_rows == 0) return 0;
+    // items of a sequence of n rows: at most (n + 30) / 32 + 1, and one for one row
+    const uint64_t most = b.starts ? (uint64_t)b.n_rows / kBlock + 2ull * std::min(v.n_seqs, b.n_rows)
+                          : b.lens ? b.n_rows : b.n_rows / kBlock + 2u;
+    const dim3 grid((uint32_t)most, v.n_heads, 2);
+    if (v.dp <= 128) hipLaunchKernelGGL(write_k<1>, grid, dim3(256), 0, st, v, b, k, x);
+    else hipLaunchKernelGGL(write_k<2>, grid, dim3(256), 0, st, v, b, k, x);
+    return launched();
+}
+
+int launch_read(const View &v, uint32_t seq, uint32_t n_seqs, uint32_t pos, uint32_t n, const Rows *k, const Rows *x,
+                hipStream_t st)
+{
+    if (n == 0 || n_seqs == 0 || (!k && !x)) return 0;
+    const uint32_t blocks = (pos + n - 1) / kBlock - pos / kBlock + 1;
+    hipLaunchKernelGGL(read_k, dim3(blocks, v.n_heads * ((k ? 1u : 0u) + (x ? 1u : 0u)), n_seqs), dim3(256), 0, st, v, seq,
+                       pos, n, k ? *k : Rows{}, x ? *x : Rows{});
+    return launched();
+}
+
+}  // namespace qg8
+
+// ------------------------------------------------------------------- C ABI
+
+namespace {
+
+// One of the context's caches.
+int check_kv8(qg_ctx *ctx, const qg_kv8 *kv)
+{
+    if (!ctx || !kv) return qg_fail(ctx, QG_ERR_INVALID_ARG, "ctx or cache is NULL");
+    if (!ctx->kv8s.count(const_cast<qg_kv8 *>(kv))) return qg_fail(ctx, QG_ERR_INVALID_ARG, "not a cache of this context");
+    return QG_OK;
+}
+
+// a * b + c in 62 bits
+bool fits(size_t a, size_t b, size_t c, size_t *out)
+{
+    size_t t;
+    if (__builtin_mul_overflow(a, b, &t) || __builtin_add_overflow(t, c, &t) || t >> 58) return false;
+    *out = t;
+    return true;
+}
+
+// qg_rows of n rows of `heads` heads of hd elements
+int check_rows(qg_ctx *ctx, const qg_rows *r, size_t n, size_t heads, size_t hd, bool written, qg8::Rows *out)
+{
+    if (!r) return qg_fail(ctx, QG_ERR_INVALID_ARG, "rows are NULL");
+    if (r->type != qg::T_F32 && r->type != qg::T_F16)
+        return qg_fail(ctx, QG_ERR_UNSUPPORTED_TYPE, "rows are neither f32 nor f16");
+    const size_t es = r->type == qg::T_F16 ? 2 : 4;
+    if (n && !r->data) return qg_fail(ctx, QG_ERR_INVALID_ARG, "rows without data");
+    if ((uintptr_t)r->data % es) return qg_fail(ctx, QG_ERR_INVALID_ARG, "rows not aligned to their elements");
+    size_t by_head, all;
+    if (!fits(heads - 1, r->ld_head, hd, &by_head) || !fits(n ? n - 1 : 0, r->ld_row, by_head, &all))
+        return qg_fail(ctx, QG_ERR_SHAPE, "rows too large");
+    if (written && n) {
+        size_t by_row;
+        const bool heads_in_rows = (heads == 1 || r->ld_head >= hd) && (n == 1 || r->ld_row >= by_head);
+        const bool rows_in_heads = fits(n - 1, r->ld_row, hd, &by_row) && (n == 1 || r->ld_row >= hd) &&
+                                   (heads == 1 || r->ld_head >= by_row);
+        if (!heads_in_rows && !rows_in_heads) return qg_fail(ctx, QG_ERR_SHAPE, "written rows overlap");
+    }
+    const size_t per = 16 / es;
+    out->p = r->data;
+    out->ld_row = r->ld_row;
+    out->ld_head = r->ld_head;
+    out->f16 = r->type == qg::T_F16;
+    out->vec = (uintptr_t)r->data % 16 == 0 && r->ld_row % per == 0 && r->ld_head % per == 0 && hd % 16 == 0;
+    return QG_OK;
+}
+
+int check_batch(qg_ctx *ctx, const qg_kv8 *kv, const qg_batch *b, qg8::Batch *out)
+{
+    if (!b) return qg_fail(ctx, QG_ERR_INVALID_ARG, "batch is NULL");
+    if (b->n_rows > 0x7FFFFFFFu) return qg_fail(ctx, QG_ERR_SHAPE, "too many rows");
+    if (!b->d_lens || ((uintptr_t)b->d_lens | (uintptr_t)b->d_starts) % 4)
+        return qg_fail(ctx, QG_ERR_INVALID_ARG, "batch lengths missing or not aligned");
+    if (!b->d_starts && b->n_rows != kv->v.n_seqs)
+        return qg_fail(ctx, QG_ERR_SHAPE, "without starts a batch has one row per sequence");
+    *out = qg8::Batch{b->d_starts, b->d_lens, (uint32_t)b->n_rows, 0};
+    return QG_OK;
+}
+
+hipStream_t pick(qg_ctx *ctx, void *stream)
+{
+    return stream ? (hipStream_t)stream : ctx->stream;
+}
+
+int launch_status(qg_ctx *ctx, int r, const char *what)
+{
+    return r == 0 ? QG_OK : qg_fail(ctx, QG_ERR_HIP, what, hipGetLastError());
+}
+
+}  // namespace
+
+int qg_kv8_make(qg_ctx *ctx, size_t n_seqs, size_t n_kv_heads, size_t head_dim, size_t max_len, qg_kv8 **out)
+{
+    if (n_seqs < 1 || n_seqs > 65535 || n_kv_heads < 1 || n_kv_heads > 65535 || head_dim < 1 || head_dim > 256 ||
+        max_len < 1 || max_len > 0x7FFFFFE0u || n_seqs * n_kv_heads > 0x3FFFFFFFu)
+        return qg_fail(ctx, QG_ERR_SHAPE, "cache sizes");
+    qg8::View v{};
+    v.n_seqs = (uint32_t)n_seqs;
+    v.n_heads = (uint32_t)n_kv_heads;
+    v.hd = (uint32_t)head_dim;
+    v.dp = (v.hd + 63u) / 64u * 64u;
+    v.max_len = (uint32_t)max_len;
+    v.n_blocks = (v.max_len + qg8::kBlock - 1) / qg8::kBlock;
+    const size_t sh = 2 * n_seqs * n_kv_heads, block = (size_t)qg8::kBlock * v.dp;
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    size_t codes;
+    if (!fits(sh * v.n_blocks, block, 0, &codes)) return qg_fail(ctx, QG_ERR_SHAPE, "cache sizes");
+    const size_t scale = up(sh * v.n_blocks * 4), tail = up(sh * 2 * block * 4), tmax = up(sh * 2 * qg8::kBlock * 4),
+                 at = up(sh * 16);
+    const size_t bytes = codes + scale + tail + tmax + at;
+    hipError_t e = hipSetDevice(ctx->device);
+    if (e != hipSuccess) return qg_fail(ctx, QG_ERR_HIP, "hipSetDevice", e);
+    qg_kv8 *kv = new (std::nothrow) qg_kv8;
+    if (!kv) return qg_fail(ctx, QG_ERR_OUT_OF_MEMORY, "host allocation");
+    kv->ctx = ctx;
+    kv->bytes = bytes;
+    e = qg_alloc_injected(ctx) ? hipErrorOutOfMemory : hipMalloc(&kv->mem, bytes);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        delete kv;
+        return qg_fail(ctx, QG_ERR_OUT_OF_MEMORY, "hipMalloc cache", e);
+    }
+    uint8_t *p = (uint8_t *)kv->mem;
+    v.codes = p;
+    v.scale = (float *)(p += codes);
+    v.tail = (float *)(p += scale);
+    v.tail_max = (uint32_t *)(p += tail);
+    v.tail_at = (int32_t *)(p += tmax);
+    kv->v = v;
+    e = hipMemsetAsync(kv->mem, 0, bytes - at, ctx->stream);
+    if (e == hipSuccess) e = hipMemsetAsync(v.tail_at, 0xFF, at, ctx->stream);      // -1: no block
+    const hipError_t es = hipStreamSynchronize(ctx->stream);
+    if (e == hipSuccess) e = es;
+    if (e != hipSuccess) {
+        qg_kv8_drop(kv);
+        return qg_fail(ctx, QG_ERR_HIP, "clearing the cache", e);
+    }
+    *out = kv;
+    return QG_OK;
+}
+
+void qg_kv8_drop(qg_kv8 *kv)
+{
+    if (!kv) return;
+    if (kv->mem) (void)hipFree(kv->mem);
+    delete kv;
+}
+
+void qg_kv8_free_all(qg_ctx *ctx)
+{
+    for (qg_kv8 *kv : ctx->kv8s) qg_kv8_drop(kv);
+    ctx->kv8s.clear();
+}
+
+extern "C" {
+
+int qg_kv8_create(qg_ctx *ctx, size_t n_seqs, size_t n_kv_heads, size_t head_dim, size_t max_len, qg_kv8 **out)
+{
+    if (!ctx || !out) return qg_fail(ctx, QG_ERR_INVALID_ARG, "ctx or out is NULL");
+    *out = nullptr;
+    qg_kv8 *kv = nullptr;
+    const int rc = qg_kv8_make(ctx, n_seqs, n_kv_heads, head_dim, max_len, &kv);
+    if (rc) return rc;
+    try {
+        ctx->kv8s.insert(kv);
+    } catch (...) {
+        qg_kv8_drop(kv);
+        return qg_fail(ctx, QG_ERR_OUT_OF_MEMORY, "host allocation");
+    }
+    *out = kv;
+    return QG_OK;
+}
+
+int qg_kv8_free(qg_ctx *ctx, qg_kv8 *kv)
+{
+    const int rc = check_kv8(ctx, kv);
+    if (rc) return rc;
+    (void)hipSetDevice(ctx->device);
+    (void)hipStreamSynchronize(ctx->stream);
+    ctx->kv8s.erase(kv);
+    qg_kv8_drop(kv);
+    return QG_OK;
+}
+
+int qg_kv8_info(const qg_kv8 *kv, size_t *n_seqs, size_t *n_kv_heads, size_t *head_dim, size_t *max_len, size_t *bytes)
+{
+    if (!kv) return QG_ERR_INVALID_ARG;
+    if (n_seqs) *n_seqs = kv->v.n_seqs;
+    if (n_kv_heads) *n_kv_heads = kv->v.n_heads;
+    if (head_dim) *head_dim = kv->v.hd;
+    if (max_len) *max_len = kv->v.max_len;
+    if (bytes) *bytes = kv->bytes;
+    return QG_OK;
+}
+
+int qg_kv8_write_dev(qg_ctx *ctx, qg_kv8 *kv, const qg_batch *batch, const qg_rows *k, const qg_rows *v, void *stream)
+{
+    int rc = check_kv8(ctx, kv);
+    qg8::Batch b{};
+    qg8::Rows rk{}, rv{};
+    if (rc || (rc = check_batch(ctx, kv, batch, &b)) ||
+        (rc = check_rows(ctx, k, b.n_rows, kv->v.n_heads, kv->v.hd, false, &rk)) ||
+        (rc = check_rows(ctx, v, b.n_rows, kv->v.n_heads, kv->v.hd, false, &rv)))
+        return rc;
+    if (rk.f16 != rv.f16) return qg_fail(ctx, QG_ERR_UNSUPPORTED_TYPE, "k and v of two types");
+    if (b.n_rows == 0) return QG_OK;
+    const hipError_t e = hipSetDevice(ctx->device);
+    if (e != hipSuccess) return qg_fail(ctx, QG_ERR_HIP, "hipSetDevice", e);
+    return launch_status(ctx, qg8::launch_write(kv->v, b, rk, rv, pick(ctx, stream)), "cache write");
+}
+
+int qg_kv8_read_dev(qg_ctx *ctx, const qg_kv8 *kv, size_t seq, size_t n_seqs, size_t pos, size_t n, const qg_rows *k,
+                    const qg_rows *v, void *stream)
+{
+    int rc = check_kv8(ctx, kv);
+    if (rc) return rc;
+    const qg8::View &c = kv->v;
+    if (seq > c.n_seqs || n_seqs > c.n_seqs - seq || pos > c.max_len || n > c.max_len - pos)
+        return qg_fail(ctx, QG_ERR_SHAPE, "positions outside the cache");
+    qg8::Rows rk{}, rv{};
+    if ((k && (rc = check_rows(ctx, k, n_seqs * n, c.n_heads, c.hd, true, &rk))) ||
+        (v && (rc = check_rows(ctx, v, n_seqs * n, c.n_heads, c.hd, true, &rv))))
+        return rc;
+    if (n == 0 || n_seqs == 0 || (!k && !v)) return QG_OK;
+    if (c.n_heads * 2ull > 65535) return qg_fail(ctx, QG_ERR_SHAPE, "too many heads to read at once");
+    const hipError_t e = hipSetDevice(ctx->device);
+    if (e != hipSuccess) return qg_fail(ctx, QG_ERR_HIP, "hipSetDevice", e);
+    return launch_status(ctx, qg8::launch_read(c, (uint32_t)seq, (uint32_t)n_seqs, (uint32_t)pos, (uint32_t)n,
+                                               k ? &rk : nullptr, v ? &rv : nullptr, pick(ctx, stream)), "cache read");
+}
+
+int qg_kv8_attention_work(qg_ctx *ctx, const qg_kv8 *kv, size_t n_rows, size_t n_heads, size_t *bytes)
+{
+    const int rc = check_kv8(ctx, kv);
+    if (rc) return rc;
+    if (!bytes) return qg_fail(ctx, QG_ERR_INVALID_ARG, "bytes is NULL");
+    if (n_rows > 0x7FFFFFFFu || n_heads == 0 || n_heads % kv->v.n_heads || n_heads > 65535)
+        return qg_fail(ctx, QG_ERR_SHAPE, "rows or heads");
+    *bytes = qg8::attention_work(kv->v, n_rows, n_heads, ctx->n_cu);
+    return QG_OK;
+}
+
+int qg_kv8_attention_dev(qg_ctx *ctx, const qg_kv8 *kv, const qg_batch *batch, size_t n_heads, const qg_rows *q,
+                         float scale, size_t window, const qg_rows *out, void *d_work, size_t work_bytes, void *stream)
+{
+    int rc = check_kv8(ctx, kv);
+    if (rc) return rc;
+    if (n_heads == 0 || n_heads % kv->v.n_heads || n_heads > 65535)
+        return qg_fail(ctx, QG_ERR_SHAPE, "query heads are no multiple of the cache's heads");
+    qg8::Batch b{};
+    qg8::Rows rq{}, ro{};
+    if ((rc = check_batch(ctx, kv, batch, &b)) || (rc = check_rows(ctx, q, b.n_rows, n_heads, kv->v.hd, false, &rq)) ||
+        (rc = check_rows(ctx, out, b.n_rows, n_heads, kv->v.hd, true, &ro)))
+        return rc;
+    if (rq.f16 != ro.f16) return qg_fail(ctx, QG_ERR_UNSUPPORTED_TYPE, "q and out of two types");
+    if (b.n_rows == 0) return QG_OK;
+    const size_t need = qg8::attention_work(kv->v, b.n_rows, n_heads, ctx->n_cu);
+    if (need > work_bytes) return qg_fail(ctx, QG_ERR_SHAPE, "workspace too small");
+    if (need && (!d_work || (uintptr_t)d_work % 16))
+        return qg_fail(ctx, QG_ERR_INVALID_ARG, "workspace missing or not 16-byte aligned");
+    const hipError_t e = hipSetDevice(ctx->device);
+    if (e != hipSuccess) return qg_fail(ctx, QG_ERR_HIP, "hipSetDevice", e);
+    // no row stands at 2^32 or above: a wider window hides nothing
+    const uint32_t win = window > 0xFFFFFFFFull ? 0u : (uint32_t)window;
+    return launch_status(ctx, qg8::launch_attention(kv->v, b, (uint32_t)n_heads, rq, scale, win, ro, d_work, ctx->n_cu,
+                                                    pick(ctx, stream)), "attention");
+}
+
+}  // extern "C"

@@ -528,6 +528,7 @@ int qg_destroy(qg_ctx *ctx)
     (void)hipSetDevice(ctx->device);
     (void)hipStreamSynchronize(ctx->stream);
     while (!ctx->mats.empty()) drop_mat(ctx, *ctx->mats.begin());
+    qg_kv8_free_all(ctx);
     if (ctx->h_x) (void)hipHostFree(ctx->h_x);
     if (ctx->h_y) (void)hipHostFree(ctx->h_y);
     if (ctx->d_x) (void)hipFree(ctx->d_x);
