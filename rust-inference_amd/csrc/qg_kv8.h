@@ -11,6 +11,8 @@
 namespace qg8 {
 
 constexpr uint32_t kBlock = QG_KV8_BLOCK;
+constexpr int kZero = 128;                   // a code's byte is the code + 128 (qg_kv8_attention.hip, halves)
+constexpr uint32_t kZeros = 0x80808080u;
 
 // A cache as the kernels see it.  A head's elements are padded with zeros to
 // dp, a multiple of 64.  Index sh = seq * n_heads + head.

@@ -115,7 +115,7 @@ __device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint6
             for (int j = 0; j < 16; j++) val[i][j] = 0.f;
             if (old && !held)          // a block reopened from its codes
                 for (uint32_t j = 0; j < 16; j++) {
-                    const int8_t q = (int8_t)codes[key ? key_at(t, d + j, dp) : value_at(t, d + j)];
+                    const int q = (int)codes[key ? key_at(t, d + j, dp) : value_at(t, d + j)] - kZero;
                     val[i][j] = (float)q * s_old;
                 }
         }
@@ -157,10 +157,10 @@ __device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint6
         const uint32_t d = 16u * (c + 8u * i);
         if (d >= dp) break;
         union { uint8_t b[16]; uint4 u; } w;
-        w.u = make_uint4(0, 0, 0, 0);
+        w.u = make_uint4(kZeros, kZeros, kZeros, kZeros);
         if (s > 0.f && put)
 #pragma unroll
-            for (int j = 0; j < 16; j++) w.b[j] = (uint8_t)(int8_t)code_of(val[i][j], s, inv);
+            for (int j = 0; j < 16; j++) w.b[j] = (uint8_t)(code_of(val[i][j], s, inv) + kZero);
         if (key) {
             if (put) *(uint4 *)(codes + key_at(t, d, dp)) = w.u;
         } else if (whole) {
@@ -275,8 +275,9 @@ __global__ void __launch_bounds__(256) read_k(View v, uint32_t seq0, uint32_t po
         return (out + (p0 + t - pos)) * x.ld_row + head * x.ld_head + d;
     };
     for (uint32_t u = threadIdx.x; u < 2 * dp; u += 256) {
-        union { int8_t b[16]; uint4 u; } w;
+        union { uint8_t b[16]; uint4 u; } w;
         w.u = *(const uint4 *)(codes + u * 16u);
+        auto val_of = [&](int j) { return (float)((int)w.b[j] - kZero) * s; };
         if (key) {
             // unit u of 16 bytes: position and 16 elements
             const uint32_t t = (u >> 6) / (dp >> 6) * 16u + (u & 15u), d = (u >> 6) % (dp >> 6) * 64u + (u >> 4 & 3u) * 16u;
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(256) read_k(View v, uint32_t seq0, uint32_t po
                 if (x.f16) {
                     union { _Float16 h[16]; uint4 u[2]; } y;
 #pragma unroll
-                    for (int j = 0; j < 16; j++) y.h[j] = (_Float16)((float)w.b[j] * s);
+                    for (int j = 0; j < 16; j++) y.h[j] = (_Float16)val_of(j);
                     uint4 *o = (uint4 *)((_Float16 *)x.p + at(t, d));
                     o[0] = y.u[0];
                     o[1] = y.u[1];
@@ -293,12 +294,11 @@ __global__ void __launch_bounds__(256) read_k(View v, uint32_t seq0, uint32_t po
                     float4 *o = (float4 *)((float *)x.p + at(t, d));
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        o[j] = make_float4((float)w.b[4 * j] * s, (float)w.b[4 * j + 1] * s, (float)w.b[4 * j + 2] * s,
-                                           (float)w.b[4 * j + 3] * s);
+                        o[j] = make_float4(val_of(4 * j), val_of(4 * j + 1), val_of(4 * j + 2), val_of(4 * j + 3));
                 }
             } else {
                 for (uint32_t j = 0; j < 16; j++)
-                    if (d + j < v.hd) store1(x, at(t, d + j), (float)w.b[j] * s);
+                    if (d + j < v.hd) store1(x, at(t, d + j), val_of((int)j));
             }
         } else {
             const uint32_t g = u >> 4 & 3u, d = (u >> 6) * 32u + 2u * (u & 15u);
@@ -306,8 +306,8 @@ __global__ void __launch_bounds__(256) read_k(View v, uint32_t seq0, uint32_t po
             for (uint32_t j = 0; j < 8; j++) {
                 const uint32_t t = 4u * g + (j & 3u) + (j >> 2) * 16u;
                 if (p0 + t < pos || p0 + t >= (uint64_t)pos + n) continue;
-                if (d < v.hd) store1(x, at(t, d), (float)w.b[j] * s);
-                if (d + 1 < v.hd) store1(x, at(t, d + 1), (float)w.b[8 + j] * s);
+                if (d < v.hd) store1(x, at(t, d), val_of((int)j));
+                if (d + 1 < v.hd) store1(x, at(t, d + 1), val_of(8 + (int)j));
             }
         }
     }
@@ -455,7 +455,8 @@ int qg_kv8_make(qg_ctx *ctx, size_t n_seqs, size_t n_kv_heads, size_t head_dim, 
     v.tail_max = (uint32_t *)(p += tail);
     v.tail_at = (int32_t *)(p += tmax);
     kv->v = v;
-    e = hipMemsetAsync(kv->mem, 0, bytes - at, ctx->stream);
+    e = hipMemsetAsync(kv->mem, qg8::kZero, codes, ctx->stream);
+    if (e == hipSuccess) e = hipMemsetAsync(v.scale, 0, bytes - at - codes, ctx->stream);
     if (e == hipSuccess) e = hipMemsetAsync(v.tail_at, 0xFF, at, ctx->stream);      // -1: no block
     const hipError_t es = hipStreamSynchronize(ctx->stream);
     if (e == hipSuccess) e = es;

@@ -1,89 +1,700 @@
 // qg_kv8_attention.hip -- attention over the 8-bit KV cache (include/qgops.h).
+//
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(s_j - m),  s_j = scale log2(e) q . k_j,
+//   k_j = ks c_j, v_j = vs d_j: codes c, d under the scales of j's block.
+//
+// One pass over the positions with a running reference m of every row.  The
+// products run on v_mfma_f32_16x16x32_f16: the codes are exact in f16, and q, p
+// are f16 pieces (one for f16 rows, hi + lo for f32 rows: 22 bits).  Both
+// products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that a lane
+// holds one row's scores (column l % 16 of S^T) in the places in which the second
+// product wants them (its B operand), and row statistics need no broadcast; the
+// cache is laid out so that a lane's 16-byte load is the A operand of two
+// products of either kind (qg_kv8.h).
+//
+//   * q is scaled by a power of two per row (largest magnitude into [1024,
+//     2048)), its sign by that of `scale`; s = f acc with one factor f >= 0 per row
+//     and block.
+//   * m moves only when a score passes it by more than kLift (then the row's sums
+//     are rescaled): no cross-lane step otherwise.  p = 2^(s - m + kBias) lies as
+//     high in f16's range as it can, for the low pieces' bits.
+//   * vs goes into p as a ratio to a running reference scale that moves only when
+//     the ratio leaves 2^-6 .. 2, so the accumulators are not touched per block.
+//   * masked positions: p = 0 whatever their codes; a NaN scale (non-finite block)
+//     reaches the rows that see a position of the block.
+//
+// Rows are (token, query head) pairs of one kv head: pair r of a sequence is token
+// r / n_rep, head r % n_rep.  Tiles of kM pairs of one sequence and kv head are the
+// items; an item's work is its visible blocks in chunks of kChunk.  All items'
+// chunks, end to end, are dealt out evenly to the workgroups (about two per
+// compute unit) whatever the sequences' lengths; a workgroup's share may end
+// inside an item, then the parts' (m, sum, unnormalised output) go to the
+// workspace and merge_k joins them.
 #include "qg_kv8.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace qg8 {
 namespace {
 
-// One wave per (row, query head): lane (t, half) scores position t of a block
-// over half of the head's elements, then lanes hold output elements.  The
-// softmax's running maximum and sum are kept in the exponent's base 2.
-__global__ void __launch_bounds__(64) row_k(View v, Batch b, uint32_t n_rep, Rows q, float scale2, uint32_t window, Rows out)
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kChunk = 4;                // blocks
+constexpr float kBias = 12.f, kLift = 2.f;   // 2^(12 + 2) times a ratio of 2: f16's largest power
+constexpr float kLow = -3.0e38f;              // below any score
+constexpr uint32_t kNone = 0xFFFFFFFFu;
+
+// Where a workgroup's share begins inside an item: the item and the workgroups
+// that have its first and last part.
+struct Split {
+    uint32_t first, last, seq, head, tile, pad[3];
+};
+
+struct Work {
+    Split *split;      // [workgroup]
+    float *ml;         // [workgroup][2][kM][2]
+    float *part;       // [workgroup][2][kM][dp]
+};
+
+// The blocks that a tile of pairs sees, and its chunks (one at least: rows
+// that see nothing are written too).
+struct Tile {
+    uint32_t blk0, blocks, chunks;
+};
+
+struct Problem {
+    View v;
+    Batch b;
+    Rows q, out;
+    uint32_t n_rep, window;
+    float scale2;      // |scale| log2(e)
+    float sign;
+    Work w;
+};
+
+// First position and one past the last that the token at position p sees.
+__device__ __forceinline__ void sight(const Problem &a, const Span &s, int64_t p, int64_t *lo, int64_t *hi)
 {
-    __shared__ float qs[256], ps[32];
-    const uint32_t row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, dp = v.dp;
-    uint32_t seq = 0;
-    Span s{};
-    bool found = false;
-    for (seq = 0; seq < v.n_seqs; seq++) {
-        s = span_of(b, seq);
-        if (row >= s.row && row < s.row + s.n) { found = true; break; }
+    const int64_t len = min(s.len, a.v.max_len);
+    *hi = p + 1 < len ? p + 1 : len;
+    *lo = a.window && p + 1 > (int64_t)a.window ? p + 1 - (int64_t)a.window : 0;
+}
+
+template <uint32_t M> __device__ __forceinline__ uint32_t tiles_of(const Problem &a, const Span &s)
+{
+    return (uint32_t)(((uint64_t)s.n * a.n_rep + M - 1) / M);
+}
+
+template <uint32_t M> __device__ __forceinline__ Tile tile_of(const Problem &a, const Span &s, uint32_t t)
+{
+    const uint64_t r0 = (uint64_t)t * M, r1 = min(r0 + M, (uint64_t)s.n * a.n_rep) - 1;
+    int64_t lo, hi, x, y;
+    sight(a, s, s.pos + (int64_t)(r0 / a.n_rep), &lo, &x);
+    sight(a, s, s.pos + (int64_t)(r1 / a.n_rep), &y, &hi);
+    Tile k;
+    k.blk0 = 0;
+    k.blocks = 0;
+    if (hi > lo) {
+        k.blk0 = (uint32_t)(lo / kBlock);
+        k.blocks = (uint32_t)((hi - 1) / kBlock) - k.blk0 + 1;
     }
-    if (!found) return;
-    const int64_t p = s.pos + (int64_t)(row - s.row);
-    const int64_t end = p + 1 < (int64_t)min(s.len, v.max_len) ? p + 1 : (int64_t)min(s.len, v.max_len);
-    const int64_t from = window && p + 1 > (int64_t)window ? p + 1 - (int64_t)window : 0;
-    for (uint32_t d = lane; d < dp; d += 64)
-        qs[d] = d < v.hd ? load1(q, (uint64_t)row * q.ld_row + (uint64_t)h * q.ld_head + d) : 0.f;
-    __syncthreads();
-    const uint64_t sh = (uint64_t)seq * v.n_heads + h / n_rep, all = (uint64_t)v.n_seqs * v.n_heads;
-    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t blk = from / 32; blk * 32 < end; blk++) {
-        const uint8_t *kc = v.codes + (sh * v.n_blocks + (uint64_t)blk) * 32 * dp;
-        const uint8_t *vc = v.codes + ((all + sh) * v.n_blocks + (uint64_t)blk) * 32 * dp;
-        const float ks = v.scale[sh * v.n_blocks + (uint64_t)blk], vs = v.scale[(all + sh) * v.n_blocks + (uint64_t)blk];
-        const uint32_t t = lane & 31u;
-        float x = 0.f;
-        for (uint32_t d = (lane >> 5) * (dp / 2); d < (lane >> 5) * (dp / 2) + dp / 2; d++)
-            x += qs[d] * (float)(int8_t)kc[key_at(t, d, dp)];
-        x += __shfl_xor(x, 32, 64);
-        const int64_t j = blk * 32 + t;
-        const bool seen = j >= from && j < end;
-        x = seen ? x * ks * scale2 : -INFINITY;
-        float bm = x;
-        for (int o = 16; o > 0; o >>= 1) bm = fmaxf(bm, __shfl_xor(bm, o, 64));
-        const float mn = fmaxf(m, bm);
-        const float pt = seen ? exp2f(x - mn) : 0.f;
-        const float alpha = m == mn ? 1.f : exp2f(m - mn);
-        float bs = pt;
-        for (int o = 16; o > 0; o >>= 1) bs += __shfl_xor(bs, o, 64);
-        l = l * alpha + bs;
-        m = mn;
-        __syncthreads();
-        if (lane < 32) ps[lane] = pt;
-        __syncthreads();
-        for (uint32_t i = 0; i < dp / 64; i++) {
-            const uint32_t d = lane + 64 * i;
-            float a = 0.f;
-            for (uint32_t u = 0; u < 32; u++) {
-                const int64_t ju = blk * 32 + u;
-                if (ju >= from && ju < end) a += ps[u] * ((float)(int8_t)vc[value_at(u, d)] * vs);
+    k.chunks = max(1u, (k.blocks + kChunk - 1) / kChunk);
+    return k;
+}
+
+// Chunks of all tiles of a sequence (one kv head), by the whole wave.
+template <uint32_t M> __device__ uint64_t seq_chunks(const Problem &a, const Span &s)
+{
+    const uint32_t n = tiles_of<M>(a, s), lane = threadIdx.x & 63u;
+    uint64_t c = 0;
+    for (uint32_t t = lane; t < n; t += 64) c += tile_of<M>(a, s, t).chunks;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) c += __shfl_xor((unsigned long long)c, o, 64);
+    return c;
+}
+
+// Chunks of 64 sequences from s0 on, a sequence per lane, all kv heads.
+template <uint32_t M> __device__ uint64_t lane_chunks(const Problem &a, uint32_t s0)
+{
+    const uint32_t lane = threadIdx.x & 63u, s = s0 + lane;
+    uint32_t n = 0;
+    uint64_t c = 0;
+    if (s < a.v.n_seqs) {
+        const Span p = span_of(a.b, s);
+        n = tiles_of<M>(a, p);
+        if (n == 1) c = tile_of<M>(a, p, 0).chunks;
+    }
+    uint64_t many = __ballot(n > 1);
+    while (many) {
+        const uint32_t l = (uint32_t)__ffsll((unsigned long long)many) - 1;
+        many &= many - 1;
+        const uint64_t t = seq_chunks<M>(a, span_of(a.b, s0 + l));
+        if (lane == l) c = t;
+    }
+    return c * a.v.n_heads;
+}
+
+__device__ __forceinline__ uint64_t scan64(uint64_t c)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+    for (uint32_t o = 1; o < 64; o <<= 1) {
+        const uint64_t up = __shfl_up((unsigned long long)c, o, 64);
+        if (lane >= o) c += up;
+    }
+    return c;
+}
+
+struct Item {
+    uint32_t seq, head, tile;
+    uint64_t start;                     // chunk the item begins with
+    Tile t;
+    Span s;
+};
+
+// All sequences' chunks; `first` keeps the running sums of the first 64.
+template <uint32_t M> __device__ uint64_t all_chunks(const Problem &a, uint64_t *first)
+{
+    uint64_t total = 0;
+    for (uint32_t s0 = 0; s0 < a.v.n_seqs; s0 += 64) {
+        const uint64_t c = scan64(lane_chunks<M>(a, s0));
+        if (s0 == 0) *first = c;
+        total += __shfl((unsigned long long)c, 63, 64);
+    }
+    return total;
+}
+
+// The item that holds chunk `at` (less than the total).
+template <uint32_t M> __device__ Item find(const Problem &a, uint64_t at, uint64_t first)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    Item it{};
+    uint64_t before = 0;
+    for (uint32_t s0 = 0; s0 < a.v.n_seqs; s0 += 64) {
+        const uint64_t c = s0 == 0 ? first : scan64(lane_chunks<M>(a, s0));
+        const uint64_t past = __ballot(before + c > at);
+        if (!past) {
+            before += __shfl((unsigned long long)c, 63, 64);
+            continue;
+        }
+        const uint32_t l = (uint32_t)__ffsll((unsigned long long)past) - 1;
+        const uint64_t up_to = __shfl((unsigned long long)c, (int)l, 64);
+        const uint64_t below = l ? __shfl((unsigned long long)c, (int)l - 1, 64) : 0ull;
+        it.seq = s0 + l;
+        it.s = span_of(a.b, it.seq);
+        before += below;
+        const uint64_t per_head = (up_to - below) / a.v.n_heads;
+        it.head = (uint32_t)((at - before) / per_head);
+        before += it.head * per_head;
+        const uint32_t n = tiles_of<M>(a, it.s);
+        for (uint32_t t0 = 0; t0 < n; t0 += 64) {
+            const uint32_t w = t0 + lane < n ? tile_of<M>(a, it.s, t0 + lane).chunks : 0u;
+            const uint64_t d = n == 1 ? (uint64_t)__shfl((int)w, 0, 64) : scan64(w);
+            const uint64_t in = __ballot(before + d > at);
+            if (!in) {
+                before += __shfl((unsigned long long)d, 63, 64);
+                continue;
             }
-            acc[i] = acc[i] * alpha + a;
+            const uint32_t k = (uint32_t)__ffsll((unsigned long long)in) - 1;
+            it.tile = t0 + k;
+            it.start = before + (k ? __shfl((unsigned long long)d, (int)k - 1, 64) : 0ull);
+            it.t = tile_of<M>(a, it.s, it.tile);
+            return it;
+        }
+        return it;
+    }
+    return it;
+}
+
+// Eight codes (bytes code + 128) as f16: 1024 + byte by its bits, less 1152.
+__device__ __forceinline__ h8 halves(uint32_t a, uint32_t b)
+{
+    const h2 bias = {(_Float16)1152.f, (_Float16)1152.f};
+    union { h2 p[4]; h8 v; } r;
+    r.p[0] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u)) - bias;
+    r.p[1] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u)) - bias;
+    r.p[2] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - bias;
+    r.p[3] = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - bias;
+    return r.v;
+}
+
+__device__ __forceinline__ v4f mfma(h8 a, h8 b, v4f c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A row's q in the B operand's layout: lane (r, g) holds elements 64 c + 16 g ..
+// + 16, the first eight for product 2 c, the others for 2 c + 1.
+template <int DP, int NP> struct QFrag {
+    h8 h[NP][DP / 32];
+    float f;                  // s = f * (key scale) * acc
+};
+
+// at < 0: no row
+template <int DP, int NP>
+__device__ void load_q(const Problem &a, bool valid, uint64_t at, uint32_t g, QFrag<DP, NP> &q)
+{
+    float x[DP / 64][16];
+    uint32_t m = 0;
+#pragma unroll
+    for (int c = 0; c < DP / 64; c++) {
+        if (valid) {
+            load16(a.q, at, 64u * c + 16u * g, a.v.hd, x[c]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++) x[c][j] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; j++) m = max(m, __float_as_uint(x[c][j]) & 0x7FFFFFFFu);
+    }
+    m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+    // largest magnitude into [1024, 2048): 2^up, within what keeps 2^-up and q 2^up normal
+    const int up = m >= 0x7F800000u ? 0 : min(137 - (int)(m >> 23), 110);
+    const float s = ldexpf(a.sign, up);
+    q.f = m >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : ldexpf(a.scale2, -up);
+#pragma unroll
+    for (int c = 0; c < DP / 64; c++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const float y = m >= 0x7F800000u ? 0.f : x[c][j] * s;
+            const _Float16 hi = (_Float16)y;
+            q.h[0][2 * c + j / 8][j % 8] = hi;
+            if (NP == 2) q.h[NP - 1][2 * c + j / 8][j % 8] = (_Float16)(y - (float)hi);
+        }
+}
+
+// A wave's running state for 16 rows: lane (r, g) holds row r's reference, the
+// sum over its own positions, and elements of the output.
+template <int DP> struct State {
+    v4f o[DP / 16];
+    float m, l;
+};
+
+// The scale of values that o is held in (0: none yet); the same in all lanes.
+struct Ref {
+    float ref;
+};
+
+// The ratio of vs to the reference, o rescaled where it has left its range.
+template <int DP, int NT> __device__ __forceinline__ float ratio_of(float vs, Ref &r, State<DP> *st)
+{
+    if (!(vs > 0.f)) return 1.f;                       // codes all zero, or NaN: see weigh
+    if (r.ref == 0.f) r.ref = vs;
+    float q = vs / r.ref;
+    if (!(q <= 2.f && q >= 0x1p-6f)) {
+        const float next = fmaxf(vs, r.ref * 0x1p-60f);
+        const float k = r.ref / next;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < DP / 16; i++) st[t].o[i] *= k;
+        r.ref = next;
+        q = vs / next;
+    }
+    return q;
+}
+
+// Scores acc[2] of a block's positions 4 g + i and 16 + 4 g + i into p (kBias
+// above the row's reference) and its f16 pieces times `ratio`.  lo, hi: the
+// positions of the block the row sees (masked: not all rows see all of it).
+template <int DP, int NP>
+__device__ __forceinline__ void weigh(const v4f *acc, float f, float ratio, float vs, bool masked, int32_t lo, int32_t hi, uint32_t g,
+                                      State<DP> &st, h8 *p)
+{
+    v4f x[2] = {acc[0], acc[1]};
+    uint32_t seen = 0xFFu;
+    if (masked) {
+        seen = 0;
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int32_t j = (int32_t)(16 * k + 4 * g + i);
+                const bool in = j >= lo && j < hi;
+                seen |= in ? 1u << (4 * k + i) : 0u;
+                x[k][i] = in ? x[k][i] : -3.0e38f;
+            }
+    }
+    float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                      fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3]))) * f;
+    if (!seen) top = kLow;
+    if (__any(top > st.m + kLift)) {
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float m = fmaxf(st.m, top), k = exp2_(st.m - m);
+        st.m = m;
+        st.l *= k;
+#pragma unroll
+        for (int i = 0; i < DP / 16; i++) st.o[i] *= k;
+    }
+    const float c = kBias - st.m;
+    float w[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) w[j] = exp2_(__builtin_fmaf(x[j / 4][j % 4], f, c));
+    if (masked) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) w[j] = seen >> j & 1u ? w[j] : 0.f;
+    }
+    if (vs != vs) {                                    // a block that is not finite
+#pragma unroll
+        for (int j = 0; j < 8; j++) w[j] = seen >> j & 1u ? vs : 0.f;
+    }
+    st.l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+    if (NP == 1) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) p[0][j] = (_Float16)(w[j] * ratio);
+    } else {
+        // the high piece by one instruction of its own: as a plain conversion it
+        // may be rounded with the product in one place and after it in another,
+        // and the low piece then belongs to a neighbour of it
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const float y = w[j] * ratio, z = w[j + 1] * ratio;
+            const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(y, z));
+            p[0][j] = h[0];
+            p[0][j + 1] = h[1];
+            p[NP - 1][j] = (_Float16)(y - (float)h[0]);
+            p[NP - 1][j + 1] = (_Float16)(z - (float)h[1]);
         }
     }
-    const float inv = end > from ? 1.f / l : 0.f;
-    for (uint32_t i = 0; i < dp / 64; i++) {
-        const uint32_t d = lane + 64 * i;
-        if (d < v.hd) store1(out, (uint64_t)row * out.ld_row + (uint64_t)h * out.ld_head + d, end > from ? acc[i] * inv : 0.f);
+}
+
+// Row r of a tile of M pairs: its row of q and out, and its positions.
+struct Row {
+    bool valid;
+    uint64_t row;
+    uint32_t head;
+    int64_t lo, hi;
+};
+
+template <uint32_t M> __device__ __forceinline__ Row row_of(const Problem &a, const Span &s, uint32_t head, uint32_t tile, uint32_t r)
+{
+    Row w;
+    const uint64_t pair = (uint64_t)tile * M + r;
+    w.valid = pair < (uint64_t)s.n * a.n_rep;
+    const uint64_t i = w.valid ? pair / a.n_rep : 0;
+    w.row = s.row + i;
+    w.head = head * a.n_rep + (uint32_t)(pair - i * a.n_rep);
+    if (!w.valid) w.head = 0;
+    sight(a, s, s.pos + (int64_t)i, &w.lo, &w.hi);
+    if (!w.valid) {                              // masks nothing, and is not stored
+        w.lo = 0;
+        w.hi = INT64_MAX;
     }
+    return w;
+}
+
+// n consecutive elements of an output row (n a multiple of 4, d too)
+__device__ __forceinline__ void store_row(const Rows &o, uint64_t at, uint32_t d, uint32_t hd, const float *x, int n)
+{
+    if (o.vec && d + (uint32_t)n <= hd) {
+        for (int i = 0; i < n; i += 4) {
+            if (o.f16) {
+                typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+                *(h4 *)((_Float16 *)o.p + at + d + i) = h4{(_Float16)x[i], (_Float16)x[i + 1], (_Float16)x[i + 2], (_Float16)x[i + 3]};
+            } else {
+                *(float4 *)((float *)o.p + at + d + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+            }
+        }
+    } else {
+        for (int i = 0; i < n; i++)
+            if (d + i < hd) store1(o, at + d + i, x[i]);
+    }
+}
+
+template <uint32_t M> __device__ __forceinline__ void put_split(const Problem &a, uint32_t wg, const Item *it, uint64_t per)
+{
+    if (threadIdx.x) return;
+    Split s{};
+    s.first = kNone;
+    if (it) {
+        s.first = (uint32_t)(it->start / per);
+        s.last = (uint32_t)((it->start + it->t.chunks - 1) / per);
+        s.seq = it->seq;
+        s.head = it->head;
+        s.tile = it->tile;
+    }
+    a.w.split[wg] = s;
+}
+
+// Workgroup id -> place in the order of the chunks: ids go round the 8 XCDs, and
+// neighbours in the order (the same keys and values) belong on one.
+__device__ __forceinline__ uint32_t place_of(uint32_t id, uint32_t n)
+{
+    const uint32_t each = n / 8;
+    return id < each * 8 ? (id % 8) * each + id / 8 : id;
+}
+
+// Few rows: tiles of 16 pairs.  The four waves take an item's blocks in turn, each
+// with all 16 rows and operands straight from the cache (the next block's 64 dp
+// bytes are requested before a block is used); their sums are joined in LDS.
+constexpr uint32_t kFewM = 16;
+
+template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) few_k(Problem a)
+{
+    constexpr int NK = DP / 32, NV = DP / 32;             // 16-byte loads of a lane per block
+    constexpr int LD = DP + 4;
+    __shared__ float so[4][16][LD], sm[4][16], sl[4][16];
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
+    const uint32_t wg = place_of(blockIdx.x, gridDim.x);
+    uint64_t first;
+    const uint64_t total = all_chunks<kFewM>(a, &first);
+    const uint64_t per = (total + gridDim.x - 1) / gridDim.x;
+    uint64_t at = wg * per;
+    const uint64_t end = min(at + per, total);
+    if (at >= end) {
+        put_split<kFewM>(a, wg, nullptr, per);
+        return;
+    }
+    bool begun = false;
+    const uint64_t all = (uint64_t)a.v.n_seqs * a.v.n_heads;
+    while (at < end) {
+        const Item it = find<kFewM>(a, at, first);
+        const uint32_t c0 = (uint32_t)(at - it.start), nc = (uint32_t)min((uint64_t)(it.t.chunks - c0), end - at);
+        if (!begun) {
+            put_split<kFewM>(a, wg, c0 ? &it : nullptr, per);
+            begun = true;
+        }
+        const uint64_t sh = (uint64_t)it.seq * a.v.n_heads + it.head;
+        const uint8_t *kb = a.v.codes + sh * a.v.n_blocks * (kBlock * DP) + lane * 16u;
+        const uint8_t *vb = a.v.codes + (all + sh) * a.v.n_blocks * (kBlock * DP) + lane * 16u;
+        const float *ks = a.v.scale + sh * a.v.n_blocks, *vs = a.v.scale + (all + sh) * a.v.n_blocks;
+        const uint32_t last = it.t.blk0 + min(it.t.blocks, (c0 + nc) * kChunk);
+        uint32_t blk = it.t.blk0 + c0 * kChunk + wave;
+        uint4 k[NK], v[NV];
+        float ksc = 0.f, vsc = 0.f;
+        auto fetch = [&](uint32_t b) {
+            const uint64_t off = (uint64_t)b * (kBlock * DP);
+#pragma unroll
+            for (int i = 0; i < NK; i++) k[i] = *(const uint4 *)(kb + off + i * 1024);
+#pragma unroll
+            for (int i = 0; i < NV; i++) v[i] = *(const uint4 *)(vb + off + i * 1024);
+            ksc = ks[b];
+            vsc = vs[b];
+        };
+        if (blk < last) fetch(blk);
+        const Row row = row_of<kFewM>(a, it.s, it.head, it.tile, r);
+        QFrag<DP, NP> q;
+        load_q<DP, NP>(a, row.valid, row.row * a.q.ld_row + row.head * a.q.ld_head, g, q);
+        State<DP> st;
+        st.m = kLow;
+        st.l = 0.f;
+#pragma unroll
+        for (int i = 0; i < DP / 16; i++) st.o[i] = v4f{0.f, 0.f, 0.f, 0.f};
+        Ref ref{0.f};
+        while (blk < last) {
+            uint4 kc[NK], vc[NV];
+#pragma unroll
+            for (int i = 0; i < NK; i++) kc[i] = k[i];
+#pragma unroll
+            for (int i = 0; i < NV; i++) vc[i] = v[i];
+            const float kcs = ksc, vcs = vsc;
+            if (blk + 4 < last) fetch(blk + 4);
+            v4f acc[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int c = 0; c < DP / 64; c++)
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const uint4 w = kc[t * (DP / 64) + c];
+                    const h8 x = halves(w.x, w.y), y = halves(w.z, w.w);
+#pragma unroll
+                    for (int n = 0; n < NP; n++) {
+                        acc[t] = mfma(x, q.h[n][2 * c], acc[t]);
+                        acc[t] = mfma(y, q.h[n][2 * c + 1], acc[t]);
+                    }
+                }
+            const float ratio = ratio_of<DP, 1>(vcs, ref, &st);
+            const int64_t b0 = (int64_t)blk * kBlock;
+            const bool masked = __any(row.lo > b0 || row.hi < b0 + (int64_t)kBlock);
+            const int32_t lo = row.lo > b0 ? (int32_t)min(row.lo - b0, (int64_t)kBlock) : 0;
+            const int32_t hi = row.hi > b0 ? (int32_t)min(row.hi - b0, (int64_t)kBlock) : 0;
+            h8 p[NP];
+            weigh<DP, NP>(acc, kcs * q.f, ratio, vcs, masked, lo, hi, g, st, p);
+#pragma unroll
+            for (int i = 0; i < DP / 32; i++) {
+                const h8 x = halves(vc[i].x, vc[i].y), y = halves(vc[i].z, vc[i].w);
+#pragma unroll
+                for (int n = 0; n < NP; n++) {
+                    st.o[2 * i] = mfma(x, p[n], st.o[2 * i]);
+                    st.o[2 * i + 1] = mfma(y, p[n], st.o[2 * i + 1]);
+                }
+            }
+            blk += 4;
+        }
+        // join the waves: lane (r, g) holds elements 32 i + 8 g .. + 8 of row r
+        st.l += __shfl_xor(st.l, 16, 64);
+        st.l += __shfl_xor(st.l, 32, 64);
+        __syncthreads();
+        if (g == 0) {
+            sm[wave][r] = st.m;
+            sl[wave][r] = st.l;
+        }
+#pragma unroll
+        for (int i = 0; i < DP / 32; i++) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float4 w;
+                w.x = st.o[2 * i][2 * h] * ref.ref;
+                w.y = st.o[2 * i + 1][2 * h] * ref.ref;
+                w.z = st.o[2 * i][2 * h + 1] * ref.ref;
+                w.w = st.o[2 * i + 1][2 * h + 1] * ref.ref;
+                *(float4 *)&so[wave][r][32 * i + 8 * g + 4 * h] = w;
+            }
+        }
+        __syncthreads();
+        const bool whole = c0 == 0 && nc == it.t.chunks;
+        const uint64_t slot = (uint64_t)wg * 2 + (c0 ? 0u : 1u);
+        for (uint32_t u = threadIdx.x; u < 16u * (DP / 4); u += 256) {
+            const uint32_t rr = u / (DP / 4), d = u % (DP / 4) * 4u;
+            const float m = fmaxf(fmaxf(sm[0][rr], sm[1][rr]), fmaxf(sm[2][rr], sm[3][rr]));
+            float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float e = exp2_(sm[w][rr] - m);
+                l += e * sl[w][rr];
+                const float4 o = *(const float4 *)&so[w][rr][d];
+                x[0] += e * o.x; x[1] += e * o.y; x[2] += e * o.z; x[3] += e * o.w;
+            }
+            if (whole) {
+                const Row w = row_of<kFewM>(a, it.s, it.head, it.tile, rr);
+                if (!w.valid) continue;
+                const float inv = w.hi > w.lo ? 1.f / l : 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] = w.hi > w.lo ? x[i] * inv : 0.f;
+                store_row(a.out, w.row * a.out.ld_row + w.head * a.out.ld_head, d, a.v.hd, x, 4);
+            } else {
+                *(float4 *)(a.w.part + (slot * kFewM + rr) * DP + d) = make_float4(x[0], x[1], x[2], x[3]);
+                if (d == 0) {
+                    a.w.ml[(slot * kFewM + rr) * 2] = m;
+                    a.w.ml[(slot * kFewM + rr) * 2 + 1] = l;
+                }
+            }
+        }
+        at += nc;
+    }
+}
+
+// Joins the parts of an item that workgroups first .. last hold (the first one's
+// in slot 1, the others' in slot 0).  Grid: (workgroups - 1, row groups); the
+// workgroup of the second part does it.  DP / 4 lanes take a row's elements; few
+// rows of many parts (PARTS): the other threads take parts in turn; else they
+// take rows.
+template <uint32_t M, int DP, bool PARTS> __global__ void __launch_bounds__(256) merge_k(Problem a)
+{
+    constexpr uint32_t L = DP / 4, N = 256 / L;            // 192 / 4 = 48: 5 groups, 16 lanes idle
+    __shared__ float sm[N], sl[N], so[N][DP];
+    const uint32_t wg = blockIdx.x + 1;
+    const Split s = a.w.split[wg];
+    if (s.first == kNone || s.first + 1 != wg) return;
+    const Span span = span_of(a.b, s.seq);
+    const uint32_t lane = threadIdx.x % L, grp = threadIdx.x / L, d = lane * 4;
+    const uint32_t r = PARTS ? blockIdx.y : blockIdx.y * N + grp;
+    float m = kLow, l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (grp < N && r < M)
+        for (uint32_t w = s.first + (PARTS ? grp : 0); w <= s.last; w += PARTS ? N : 1) {
+            const uint64_t at = ((uint64_t)w * 2 + (w == s.first ? 1u : 0u)) * M + r;
+            const float2 t = *(const float2 *)(a.w.ml + at * 2);
+            const float4 o = *(const float4 *)(a.w.part + at * DP + d);
+            const float n = fmaxf(m, t.x), e = exp2_(m - n), f = exp2_(t.x - n);
+            m = n;
+            l = l * e + t.y * f;
+            x.x = x.x * e + o.x * f; x.y = x.y * e + o.y * f; x.z = x.z * e + o.z * f; x.w = x.w * e + o.w * f;
+        }
+    if (PARTS) {
+        if (grp < N) {
+            if (lane == 0) { sm[grp] = m; sl[grp] = l; }
+            *(float4 *)&so[grp][d] = x;
+        }
+        __syncthreads();
+        if (grp) return;
+        for (uint32_t w = 1; w < N; w++) {
+            const float n = fmaxf(m, sm[w]), e = exp2_(m - n), f = exp2_(sm[w] - n);
+            const float4 o = *(const float4 *)&so[w][d];
+            m = n;
+            l = l * e + sl[w] * f;
+            x.x = x.x * e + o.x * f; x.y = x.y * e + o.y * f; x.z = x.z * e + o.z * f; x.w = x.w * e + o.w * f;
+        }
+    }
+    if (grp >= N || r >= M) return;
+    const Row w = row_of<M>(a, span, s.head, s.tile, r);
+    if (!w.valid) return;
+    const float inv = 1.f / l;
+    float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+    if (!(w.hi > w.lo)) y[0] = y[1] = y[2] = y[3] = 0.f;
+    store_row(a.out, w.row * a.out.ld_row + w.head * a.out.ld_head, d, a.v.hd, y, 4);
+}
+
+// Workgroups of a call, and its workspace.
+uint32_t workgroups(int n_cu)
+{
+    return 2u * (uint32_t)(n_cu > 0 ? n_cu : 256);
+}
+
+size_t work_bytes(uint32_t wgs, uint32_t m, uint32_t dp)
+{
+    return (size_t)wgs * (sizeof(Split) + 2u * m * (dp + 2u) * sizeof(float));
+}
+
+Work work_at(void *p, uint32_t wgs, uint32_t m)
+{
+    Work w;
+    w.split = (Split *)p;
+    w.ml = (float *)(w.split + wgs);
+    w.part = w.ml + (size_t)wgs * 2 * m * 2;
+    return w;
+}
+
+template <int DP> int launch_dp(Problem &a, int n_cu, hipStream_t st)
+{
+    const uint32_t wgs = workgroups(n_cu);
+    if (a.q.f16) hipLaunchKernelGGL((few_k<DP, 1>), dim3(wgs), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((few_k<DP, 2>), dim3(wgs), dim3(256), 0, st, a);
+    if (hipPeekAtLastError() != hipSuccess) return -1;
+    // no item of a cache of one chunk is ever cut
+    if (a.v.n_blocks > kChunk) {
+        const uint32_t rows = a.b.lens && !a.b.starts ? std::min(kFewM, a.n_rep) : kFewM;
+        hipLaunchKernelGGL((merge_k<kFewM, DP, true>), dim3(wgs - 1, rows), dim3(256), 0, st, a);
+    }
+    return hipPeekAtLastError() == hipSuccess ? 0 : -1;
 }
 
 }  // namespace
 
-size_t attention_work(const View &, size_t, size_t, int)
+size_t attention_work(const View &v, size_t n_rows, size_t n_heads, int n_cu)
 {
-    return 0;
+    (void)n_rows;
+    (void)n_heads;
+    return work_bytes(workgroups(n_cu), kFewM, v.dp);
 }
 
 int launch_attention(const View &v, const Batch &b, uint32_t n_heads, const Rows &q, float scale, uint32_t window,
-                     const Rows &out, void *, int, hipStream_t st)
+                     const Rows &out, void *work, int n_cu, hipStream_t st)
 {
     if (b.n_rows == 0) return 0;
-    hipLaunchKernelGGL(row_k, dim3(b.n_rows, n_heads), dim3(64), 0, st, v, b, n_heads / v.n_heads, q,
-                       scale * 1.44269504f, window, out);
-    return hipPeekAtLastError() == hipSuccess ? 0 : -1;
+    Problem a{};
+    a.v = v;
+    a.b = b;
+    a.q = q;
+    a.out = out;
+    a.n_rep = n_heads / v.n_heads;
+    a.window = window;
+    a.sign = std::signbit(scale) ? -1.f : 1.f;
+    a.scale2 = fabsf(scale) * 1.44269504f;
+    a.w = work_at(work, workgroups(n_cu), kFewM);
+    switch (v.dp) {
+    case 64: return launch_dp<64>(a, n_cu, st);
+    case 128: return launch_dp<128>(a, n_cu, st);
+    case 192: return launch_dp<192>(a, n_cu, st);
+    case 256: return launch_dp<256>(a, n_cu, st);
+    default: return -1;
+    }
 }
 
 }  // namespace qg8
