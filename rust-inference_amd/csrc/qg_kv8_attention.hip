@@ -580,6 +580,176 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
     }
 }
 
+// Many rows: tiles of 64 RT pairs, 16 RT a wave.  The workgroup's waves share
+// an item's blocks: BT at a time their codes are loaded into registers (a step
+// ahead), turned into f16 once and put into one of two LDS buffers in the order of
+// the operands, from where every wave feeds its products (a K or V operand is
+// read once for RT of them).
+template <int DP, int NP, int RT, int BT> __global__ void __launch_bounds__(256, 2) many_k(Problem a)
+{
+    constexpr uint32_t M = 64 * RT;
+    constexpr int NU = DP / 64;                           // 16-byte units of codes a thread stages per block
+    extern __shared__ __attribute__((aligned(16))) h8 stage[];        // [2][BT][keys, values][DP / 32 * 2][64]
+    constexpr uint32_t kOne = DP * 4, kBuf = BT * 2 * kOne;           // operands of 16 bytes: keys or values of a block, a buffer
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
+    const uint32_t wg = place_of(blockIdx.x, gridDim.x);
+    uint64_t first;
+    const uint64_t total = all_chunks<M>(a, &first);
+    const uint64_t per = (total + gridDim.x - 1) / gridDim.x;
+    uint64_t at = wg * per;
+    const uint64_t end = min(at + per, total);
+    if (at >= end) {
+        put_split<M>(a, wg, nullptr, per);
+        return;
+    }
+    bool begun = false;
+    const uint64_t all = (uint64_t)a.v.n_seqs * a.v.n_heads;
+    while (at < end) {
+        const Item it = find<M>(a, at, first);
+        const uint32_t c0 = (uint32_t)(at - it.start), nc = (uint32_t)min((uint64_t)(it.t.chunks - c0), end - at);
+        if (!begun) {
+            put_split<M>(a, wg, c0 ? &it : nullptr, per);
+            begun = true;
+        }
+        const uint64_t sh = (uint64_t)it.seq * a.v.n_heads + it.head;
+        const uint8_t *kb = a.v.codes + sh * a.v.n_blocks * (kBlock * DP);
+        const uint8_t *vb = a.v.codes + (all + sh) * a.v.n_blocks * (kBlock * DP);
+        const float *ks = a.v.scale + sh * a.v.n_blocks, *vs = a.v.scale + (all + sh) * a.v.n_blocks;
+        const uint32_t last = it.t.blk0 + min(it.t.blocks, (c0 + nc) * kChunk);
+        uint32_t blk = it.t.blk0 + c0 * kChunk;
+        uint4 code[BT][NU];
+        float ksc[BT], vsc[BT], ksn[BT], vsn[BT];
+        auto fetch = [&](uint32_t b) {
+#pragma unroll
+            for (int t = 0; t < BT; t++) {
+                const uint32_t bt = min(b + t, last - 1);
+                const uint64_t off = (uint64_t)bt * (kBlock * DP);
+#pragma unroll
+                for (int i = 0; i < NU; i++) {
+                    const uint32_t u = threadIdx.x + 256u * i;
+                    code[t][i] = *(const uint4 *)(u < 2 * DP ? kb + off + u * 16u : vb + off + (u - 2 * DP) * 16u);
+                }
+                ksn[t] = ks[bt];
+                vsn[t] = vs[bt];
+            }
+        };
+        auto put = [&](uint32_t buf) {
+#pragma unroll
+            for (int t = 0; t < BT; t++)
+#pragma unroll
+                for (int i = 0; i < NU; i++) {
+                    const uint32_t u = threadIdx.x + 256u * i;
+                    h8 *to = stage + buf * kBuf + t * 2 * kOne + (u >> 6) * 128u + lane;
+                    to[0] = halves(code[t][i].x, code[t][i].y);
+                    to[64] = halves(code[t][i].z, code[t][i].w);
+                }
+        };
+        if (blk < last) fetch(blk);
+        QFrag<DP, NP> q[RT];
+        State<DP> st[RT];
+        int64_t lo[RT], hi[RT];
+        int64_t lo_all = 0, hi_all = INT64_MAX;
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const Row row = row_of<M>(a, it.s, it.head, it.tile, (wave * RT + t) * 16u + r);
+            load_q<DP, NP>(a, row.valid, row.row * a.q.ld_row + row.head * a.q.ld_head, g, q[t]);
+            lo[t] = row.lo;
+            hi[t] = row.hi;
+            lo_all = max(lo_all, row.lo);
+            hi_all = min(hi_all, row.hi);
+            st[t].m = kLow;
+            st[t].l = 0.f;
+#pragma unroll
+            for (int i = 0; i < DP / 16; i++) st[t].o[i] = v4f{0.f, 0.f, 0.f, 0.f};
+        }
+        Ref ref{0.f};
+        uint32_t buf = 0;
+        if (blk < last) put(0);
+        __syncthreads();
+        for (; blk < last; blk += BT) {
+#pragma unroll
+            for (int t = 0; t < BT; t++) {
+                ksc[t] = ksn[t];
+                vsc[t] = vsn[t];
+            }
+            const bool more = blk + BT < last;
+            if (more) fetch(blk + BT);
+#pragma unroll
+            for (int t = 0; t < BT; t++) {
+                const h8 *kf = stage + buf * kBuf + t * 2 * kOne + lane, *vf = kf + kOne;
+                v4f acc[RT][2];
+#pragma unroll
+                for (int x = 0; x < RT; x++) acc[x][0] = acc[x][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < DP / 32; c++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const h8 w = kf[(k * (DP / 32) + c) * 64];
+#pragma unroll
+                        for (int x = 0; x < RT; x++)
+#pragma unroll
+                            for (int n = 0; n < NP; n++) acc[x][k] = mfma(w, q[x].h[n][c], acc[x][k]);
+                    }
+                const float ratio = ratio_of<DP, RT>(vsc[t], ref, st);
+                const int64_t b0 = (int64_t)(blk + t) * kBlock;
+                const bool none = blk + t >= last;
+                const bool masked = __any(none || lo_all > b0 || hi_all < b0 + (int64_t)kBlock);
+                h8 p[RT][NP];
+#pragma unroll
+                for (int x = 0; x < RT; x++) {
+                    const int32_t l = lo[x] > b0 ? (int32_t)min(lo[x] - b0, (int64_t)kBlock) : 0;
+                    const int32_t h = none ? 0 : hi[x] > b0 ? (int32_t)min(hi[x] - b0, (int64_t)kBlock) : 0;
+                    weigh<DP, NP>(acc[x], ksc[t] * q[x].f, ratio, vsc[t], masked, l, h, g, st[x], p[x]);
+                }
+#pragma unroll
+                for (int i = 0; i < DP / 16; i++) {
+                    const h8 w = vf[i * 64];
+#pragma unroll
+                    for (int x = 0; x < RT; x++)
+#pragma unroll
+                        for (int n = 0; n < NP; n++) st[x].o[i] = mfma(w, p[x][n], st[x].o[i]);
+                }
+            }
+            if (more) put(buf ^ 1u);
+            buf ^= 1u;
+            __syncthreads();
+        }
+        const bool whole = c0 == 0 && nc == it.t.chunks;
+        const uint64_t slot = (uint64_t)wg * 2 + (c0 ? 0u : 1u);
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const uint32_t rr = (wave * RT + t) * 16u + r;
+            float l = st[t].l;
+            l += __shfl_xor(l, 16, 64);
+            l += __shfl_xor(l, 32, 64);
+            const Row w = row_of<M>(a, it.s, it.head, it.tile, rr);
+            const float k = !whole ? ref.ref : w.hi > w.lo ? ref.ref / l : 0.f;
+            if (!whole && g == 0) {
+                a.w.ml[(slot * M + rr) * 2] = st[t].m;
+                a.w.ml[(slot * M + rr) * 2 + 1] = l;
+            }
+#pragma unroll
+            for (int i = 0; i < DP / 32; i++) {
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    x[j] = st[t].o[2 * i + (j & 1)][j >> 1] * k;
+                    if (whole && !(w.hi > w.lo)) x[j] = 0.f;
+                }
+                const uint32_t d = 32 * i + 8 * g;
+                if (!whole) {
+                    float4 *o = (float4 *)(a.w.part + (slot * M + rr) * DP + d);
+                    o[0] = make_float4(x[0], x[1], x[2], x[3]);
+                    o[1] = make_float4(x[4], x[5], x[6], x[7]);
+                } else if (w.valid) {
+                    store_row(a.out, w.row * a.out.ld_row + w.head * a.out.ld_head, d, a.v.hd, x, 8);
+                }
+            }
+        }
+        at += nc;
+    }
+}
+
 // Joins the parts of an item that workgroups first .. last hold (the first one's
 // in slot 1, the others' in slot 0).  Grid: (workgroups - 1, row groups); the
 // workgroup of the second part does it.  DP / 4 lanes take a row's elements; few
@@ -588,47 +758,44 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
 template <uint32_t M, int DP, bool PARTS> __global__ void __launch_bounds__(256) merge_k(Problem a)
 {
     constexpr uint32_t L = DP / 4, N = 256 / L;            // 192 / 4 = 48: 5 groups, 16 lanes idle
-    __shared__ float sm[N], sl[N], so[N][DP];
+    __shared__ __attribute__((aligned(16))) float sm[N], sl[N], so[N][DP];
     const uint32_t wg = blockIdx.x + 1;
     const Split s = a.w.split[wg];
     if (s.first == kNone || s.first + 1 != wg) return;
     const Span span = span_of(a.b, s.seq);
     const uint32_t lane = threadIdx.x % L, grp = threadIdx.x / L, d = lane * 4;
-    const uint32_t r = PARTS ? blockIdx.y : blockIdx.y * N + grp;
-    float m = kLow, l = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (grp < N && r < M)
-        for (uint32_t w = s.first + (PARTS ? grp : 0); w <= s.last; w += PARTS ? N : 1) {
-            const uint64_t at = ((uint64_t)w * 2 + (w == s.first ? 1u : 0u)) * M + r;
-            const float2 t = *(const float2 *)(a.w.ml + at * 2);
-            const float4 o = *(const float4 *)(a.w.part + at * DP + d);
-            const float n = fmaxf(m, t.x), e = exp2_(m - n), f = exp2_(t.x - n);
-            m = n;
-            l = l * e + t.y * f;
+    for (uint32_t r = PARTS ? blockIdx.y : blockIdx.y * N + grp; r < M; r += PARTS ? M : gridDim.y * N) {
+        float m = kLow, l = 0.f;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](float n, float k, float4 o) {
+            const float top = fmaxf(m, n), e = exp2_(m - top), f = exp2_(n - top);
+            m = top;
+            l = l * e + k * f;
             x.x = x.x * e + o.x * f; x.y = x.y * e + o.y * f; x.z = x.z * e + o.z * f; x.w = x.w * e + o.w * f;
+        };
+        if (grp < N)
+            for (uint32_t w = s.first + (PARTS ? grp : 0); w <= s.last; w += PARTS ? N : 1) {
+                const uint64_t at = ((uint64_t)w * 2 + (w == s.first ? 1u : 0u)) * M + r;
+                const float2 t = *(const float2 *)(a.w.ml + at * 2);
+                add(t.x, t.y, *(const float4 *)(a.w.part + at * DP + d));
+            }
+        if (PARTS) {
+            if (grp < N) {
+                if (lane == 0) { sm[grp] = m; sl[grp] = l; }
+                *(float4 *)&so[grp][d] = x;
+            }
+            __syncthreads();
+            if (grp) return;
+            for (uint32_t w = 1; w < N; w++) add(sm[w], sl[w], *(const float4 *)&so[w][d]);
         }
-    if (PARTS) {
-        if (grp < N) {
-            if (lane == 0) { sm[grp] = m; sl[grp] = l; }
-            *(float4 *)&so[grp][d] = x;
-        }
-        __syncthreads();
-        if (grp) return;
-        for (uint32_t w = 1; w < N; w++) {
-            const float n = fmaxf(m, sm[w]), e = exp2_(m - n), f = exp2_(sm[w] - n);
-            const float4 o = *(const float4 *)&so[w][d];
-            m = n;
-            l = l * e + sl[w] * f;
-            x.x = x.x * e + o.x * f; x.y = x.y * e + o.y * f; x.z = x.z * e + o.z * f; x.w = x.w * e + o.w * f;
-        }
+        if (grp >= N) return;
+        const Row w = row_of<M>(a, span, s.head, s.tile, r);
+        if (!w.valid) continue;
+        const float inv = 1.f / l;
+        float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+        if (!(w.hi > w.lo)) y[0] = y[1] = y[2] = y[3] = 0.f;
+        store_row(a.out, w.row * a.out.ld_row + w.head * a.out.ld_head, d, a.v.hd, y, 4);
     }
-    if (grp >= N || r >= M) return;
-    const Row w = row_of<M>(a, span, s.head, s.tile, r);
-    if (!w.valid) return;
-    const float inv = 1.f / l;
-    float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
-    if (!(w.hi > w.lo)) y[0] = y[1] = y[2] = y[3] = 0.f;
-    store_row(a.out, w.row * a.out.ld_row + w.head * a.out.ld_head, d, a.v.hd, y, 4);
 }
 
 // Workgroups of a call, and its workspace.
@@ -651,27 +818,63 @@ Work work_at(void *p, uint32_t wgs, uint32_t m)
     return w;
 }
 
-template <int DP> int launch_dp(Problem &a, int n_cu, hipStream_t st)
+// Which tiles a call takes, by its (token, head) pairs per sequence and kv
+// head: what is not a sequence's is computed for nothing, while fewer, larger
+// tiles read and convert the cache less often.
+enum Kind { kFew, kMany64, kMany128 };
+
+Kind kind_of(const View &v, uint64_t n_rows, bool starts, uint64_t n_rep)
+{
+    const uint64_t pairs = starts ? n_rows * n_rep / std::min<uint64_t>(v.n_seqs, n_rows ? n_rows : 1) : n_rep;
+    if (pairs <= 32) return kFew;
+    return pairs <= 64 || v.dp > 128 ? kMany64 : kMany128;
+}
+
+uint32_t tile_rows(Kind k)
+{
+    return k == kFew ? kFewM : k == kMany64 ? 64u : 128u;
+}
+
+template <int DP, int NP, int RT, int BT> int launch_many(Problem &a, uint32_t wgs, hipStream_t st)
+{
+    const size_t lds = 2u * BT * 2u * DP * 4u * 16u;
+    hipLaunchKernelGGL((many_k<DP, NP, RT, BT>), dim3(wgs), dim3(256), lds, st, a);
+    if (hipPeekAtLastError() != hipSuccess) return -1;
+    if (a.v.n_blocks > kChunk)
+        hipLaunchKernelGGL((merge_k<64 * RT, DP, false>), dim3(wgs - 1, 4), dim3(256), 0, st, a);
+    return hipPeekAtLastError() == hipSuccess ? 0 : -1;
+}
+
+template <int DP> int launch_dp(Problem &a, Kind kind, int n_cu, hipStream_t st)
 {
     const uint32_t wgs = workgroups(n_cu);
-    if (a.q.f16) hipLaunchKernelGGL((few_k<DP, 1>), dim3(wgs), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((few_k<DP, 2>), dim3(wgs), dim3(256), 0, st, a);
-    if (hipPeekAtLastError() != hipSuccess) return -1;
-    // no item of a cache of one chunk is ever cut
-    if (a.v.n_blocks > kChunk) {
-        const uint32_t rows = a.b.lens && !a.b.starts ? std::min(kFewM, a.n_rep) : kFewM;
-        hipLaunchKernelGGL((merge_k<kFewM, DP, true>), dim3(wgs - 1, rows), dim3(256), 0, st, a);
+    if (kind == kFew) {
+        if (a.q.f16) hipLaunchKernelGGL((few_k<DP, 1>), dim3(wgs), dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((few_k<DP, 2>), dim3(wgs), dim3(256), 0, st, a);
+        if (hipPeekAtLastError() != hipSuccess) return -1;
+        // no item of a cache of one chunk is ever cut
+        if (a.v.n_blocks > kChunk) {
+            const uint32_t rows = a.b.lens && !a.b.starts ? std::min(kFewM, a.n_rep) : kFewM;
+            hipLaunchKernelGGL((merge_k<kFewM, DP, true>), dim3(wgs - 1, rows), dim3(256), 0, st, a);
+        }
+        return hipPeekAtLastError() == hipSuccess ? 0 : -1;
     }
-    return hipPeekAtLastError() == hipSuccess ? 0 : -1;
+    constexpr int BT = DP <= 128 ? 2 : 1;
+    if (kind == kMany64)
+        return a.q.f16 ? launch_many<DP, 1, 1, BT>(a, wgs, st) : launch_many<DP, 2, 1, BT>(a, wgs, st);
+    if constexpr (DP <= 128)
+        return a.q.f16 ? launch_many<DP, 1, 2, BT>(a, wgs, st) : launch_many<DP, 2, 2, BT>(a, wgs, st);
+    return -1;
 }
 
 }  // namespace
 
 size_t attention_work(const View &v, size_t n_rows, size_t n_heads, int n_cu)
 {
-    (void)n_rows;
-    (void)n_heads;
-    return work_bytes(workgroups(n_cu), kFewM, v.dp);
+    // calls of fewer rows take no larger tiles
+    const uint32_t m = std::max(tile_rows(kind_of(v, n_rows, true, n_heads / v.n_heads)),
+                                tile_rows(kind_of(v, n_rows, false, n_heads / v.n_heads)));
+    return work_bytes(workgroups(n_cu), m, v.dp);
 }
 
 int launch_attention(const View &v, const Batch &b, uint32_t n_heads, const Rows &q, float scale, uint32_t window,
@@ -687,12 +890,13 @@ int launch_attention(const View &v, const Batch &b, uint32_t n_heads, const Rows
     a.window = window;
     a.sign = std::signbit(scale) ? -1.f : 1.f;
     a.scale2 = fabsf(scale) * 1.44269504f;
-    a.w = work_at(work, workgroups(n_cu), kFewM);
+    const Kind kind = kind_of(v, b.n_rows, b.starts || !b.lens, a.n_rep);
+    a.w = work_at(work, workgroups(n_cu), tile_rows(kind));
     switch (v.dp) {
-    case 64: return launch_dp<64>(a, n_cu, st);
-    case 128: return launch_dp<128>(a, n_cu, st);
-    case 192: return launch_dp<192>(a, n_cu, st);
-    case 256: return launch_dp<256>(a, n_cu, st);
+    case 64: return launch_dp<64>(a, kind, n_cu, st);
+    case 128: return launch_dp<128>(a, kind, n_cu, st);
+    case 192: return launch_dp<192>(a, kind, n_cu, st);
+    case 256: return launch_dp<256>(a, kind, n_cu, st);
     default: return -1;
     }
 }
