@@ -563,7 +563,7 @@ int qg_kv8_attention_work(qg_ctx *ctx, const qg_kv8 *kv, size_t n_rows, size_t n
     const int rc = check_kv8(ctx, kv);
     if (rc) return rc;
     if (!bytes) return qg_fail(ctx, QG_ERR_INVALID_ARG, "bytes is NULL");
-    if (n_rows > 0x7FFFFFFFu || n_heads == 0 || n_heads % kv->v.n_heads || n_heads > 65535)
+    if (n_heads == 0 || n_heads % kv->v.n_heads || n_heads > 65535 || n_rows > 0x7FFFFFFFu / (n_heads / kv->v.n_heads))
         return qg_fail(ctx, QG_ERR_SHAPE, "rows or heads");
     *bytes = qg8::attention_work(kv->v, n_rows, n_heads, ctx->n_cu);
     return QG_OK;
@@ -581,6 +581,7 @@ int qg_kv8_attention_dev(qg_ctx *ctx, const qg_kv8 *kv, const qg_batch *batch, s
     if ((rc = check_batch(ctx, kv, batch, &b)) || (rc = check_rows(ctx, q, b.n_rows, n_heads, kv->v.hd, false, &rq)) ||
         (rc = check_rows(ctx, out, b.n_rows, n_heads, kv->v.hd, true, &ro)))
         return rc;
+    if (b.n_rows > 0x7FFFFFFFu / (n_heads / kv->v.n_heads)) return qg_fail(ctx, QG_ERR_SHAPE, "too many rows");
     if (rq.f16 != ro.f16) return qg_fail(ctx, QG_ERR_UNSUPPORTED_TYPE, "q and out of two types");
     if (b.n_rows == 0) return QG_OK;
     const size_t need = qg8::attention_work(kv->v, b.n_rows, n_heads, ctx->n_cu);

@@ -24,7 +24,7 @@
 //     reaches the rows that see a position of the block.
 //
 // Rows are (token, query head) pairs of one kv head: pair r of a sequence is token
-// r / n_rep, head r % n_rep.  Tiles of kM pairs of one sequence and kv head are the
+// r / n_rep, head r % n_rep (the callers keep n_rows * n_rep below 2^31).  Tiles of kM pairs of one sequence and kv head are the
 // items; an item's work is its visible blocks in chunks of kChunk.  All items'
 // chunks, end to end, are dealt out evenly to the workgroups (about two per
 // compute unit) whatever the sequences' lengths; a workgroup's share may end
@@ -34,6 +34,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace qg8 {
 namespace {
@@ -85,12 +86,12 @@ __device__ __forceinline__ void sight(const Problem &a, const Span &s, int64_t p
 
 template <uint32_t M> __device__ __forceinline__ uint32_t tiles_of(const Problem &a, const Span &s)
 {
-    return (uint32_t)(((uint64_t)s.n * a.n_rep + M - 1) / M);
+    return (s.n * a.n_rep + M - 1) / M;
 }
 
 template <uint32_t M> __device__ __forceinline__ Tile tile_of(const Problem &a, const Span &s, uint32_t t)
 {
-    const uint64_t r0 = (uint64_t)t * M, r1 = min(r0 + M, (uint64_t)s.n * a.n_rep) - 1;
+    const uint32_t r0 = t * M, r1 = min(r0 + M, s.n * a.n_rep) - 1;
     int64_t lo, hi, x, y;
     sight(a, s, s.pos + (int64_t)(r0 / a.n_rep), &lo, &x);
     sight(a, s, s.pos + (int64_t)(r1 / a.n_rep), &y, &hi);
@@ -276,93 +277,105 @@ template <int DP> struct State {
     float m, l;
 };
 
-// The scale of values that o is held in (0: none yet); the same in all lanes.
+// The scale of values that o is held in (0: none yet) and its inverse; the same
+// in all lanes.
 struct Ref {
-    float ref;
+    float ref, inv;
 };
 
-// The ratio of vs to the reference, o rescaled where it has left its range.
-template <int DP, int NT> __device__ __forceinline__ float ratio_of(float vs, Ref &r, State<DP> *st)
+// Keeps the largest of the next blocks' scales within 2^-6 .. 2 of the reference;
+// o is rescaled where it is not.
+template <int DP, int NT> __device__ __forceinline__ void refer(float vs, Ref &r, State<DP> *st)
 {
-    if (!(vs > 0.f)) return 1.f;                       // codes all zero, or NaN: see weigh
-    if (r.ref == 0.f) r.ref = vs;
-    float q = vs / r.ref;
-    if (!(q <= 2.f && q >= 0x1p-6f)) {
-        const float next = fmaxf(vs, r.ref * 0x1p-60f);
-        const float k = r.ref / next;
+    const float q = vs * r.inv;
+    if ((q <= 2.f && q >= 0x1p-6f) || !(vs > 0.f)) return;
+    const float next = r.ref > 0.f ? fmaxf(vs, r.ref * 0x1p-60f) : vs, k = r.ref / next;
 #pragma unroll
-        for (int t = 0; t < NT; t++)
+    for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int i = 0; i < DP / 16; i++) st[t].o[i] *= k;
-        r.ref = next;
-        q = vs / next;
-    }
-    return q;
+        for (int i = 0; i < DP / 16; i++) st[t].o[i] *= k;
+    r.ref = next;
+    r.inv = 1.f / next;
 }
 
-// Scores acc[2] of a block's positions 4 g + i and 16 + 4 g + i into p (kBias
-// above the row's reference) and its f16 pieces times `ratio`.  lo, hi: the
-// positions of the block the row sees (masked: not all rows see all of it).
-template <int DP, int NP>
-__device__ __forceinline__ void weigh(const v4f *acc, float f, float ratio, float vs, bool masked, int32_t lo, int32_t hi, uint32_t g,
-                                      State<DP> &st, h8 *p)
+// vs / ref as a power of two, and inverted.  A scale of 0 (all codes zero) or NaN
+// (see weigh) counts as 1; one that is nothing beside the reference as 2^-100,
+// which f16 does not hold either.
+__device__ __forceinline__ void ratio_of(float vs, const Ref &r, float *log, float *inv)
 {
-    v4f x[2] = {acc[0], acc[1]};
-    uint32_t seen = 0xFFu;
-    if (masked) {
-        seen = 0;
+    const float q = vs > 0.f ? fmaxf(vs * r.inv, 0x1p-100f) : 1.f;
+    *log = __builtin_amdgcn_logf(q);
+    *inv = __builtin_amdgcn_rcpf(q);
+}
+
+// Which of a block's positions 4 g + i and 16 + 4 g + i a row sees that sees lo
+// .. hi of it: bit 4 k + i.
+__device__ __forceinline__ uint32_t seen_of(int32_t lo, int32_t hi, uint32_t g)
+{
+    uint32_t s = 0;
 #pragma unroll
-        for (int k = 0; k < 2; k++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int32_t j = (int32_t)(16 * k + 4 * g + i);
-                const bool in = j >= lo && j < hi;
-                seen |= in ? 1u << (4 * k + i) : 0u;
-                x[k][i] = in ? x[k][i] : -3.0e38f;
-            }
+    for (int j = 0; j < 8; j++) {
+        const int32_t at = (int32_t)(16 * (j / 4) + 4 * g) + j % 4;
+        s |= at >= lo && at < hi ? 1u << j : 0u;
     }
-    float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
-                      fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3]))) * f;
-    if (!seen) top = kLow;
-    if (__any(top > st.m + kLift)) {
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float m = fmaxf(st.m, top), k = exp2_(st.m - m);
-        st.m = m;
-        st.l *= k;
+    return s;
+}
+
+// Largest of a lane's eight scores.
+__device__ __forceinline__ float top_of(const v4f *x)
+{
+    return fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+}
+
+// Moves the rows' references up where `top` (a lane's largest score) is past them.
+template <int DP> __device__ __forceinline__ void lift(float top, State<DP> &st)
+{
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float m = fmaxf(st.m, top), k = exp2_(st.m - m);
+    st.m = m;
+    st.l *= k;
 #pragma unroll
-        for (int i = 0; i < DP / 16; i++) st.o[i] *= k;
-    }
-    const float c = kBias - st.m;
+    for (int i = 0; i < DP / 16; i++) st.o[i] *= k;
+}
+
+// A block's scores x into p, kBias above the row's reference, and its f16
+// pieces.  log, inv: the block's ratio (2^log, 1 / it).  SOME: positions outside
+// `seen` weigh nothing, and where `nan` is set the others weigh NaN.
+template <int DP, int NP, bool SOME>
+__device__ __forceinline__ void weigh(const v4f *x, float f, float log, float inv, uint32_t seen, bool nan, State<DP> &st, h8 *p)
+{
+    const float c = kBias - st.m + log;
     float w[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) w[j] = exp2_(__builtin_fmaf(x[j / 4][j % 4], f, c));
-    if (masked) {
+    if (SOME) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) w[j] = seen >> j & 1u ? w[j] : 0.f;
+        for (int j = 0; j < 8; j++) w[j] = seen >> j & 1u ? (nan ? __uint_as_float(0x7FC00000u) : w[j]) : 0.f;
     }
-    if (vs != vs) {                                    // a block that is not finite
-#pragma unroll
-        for (int j = 0; j < 8; j++) w[j] = seen >> j & 1u ? vs : 0.f;
-    }
-    st.l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+    st.l = __builtin_fmaf(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])), inv, st.l);
     if (NP == 1) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) p[0][j] = (_Float16)(w[j] * ratio);
+        for (int j = 0; j < 8; j++) p[0][j] = (_Float16)w[j];
     } else {
-        // the high piece by one instruction of its own: as a plain conversion it
-        // may be rounded with the product in one place and after it in another,
-        // and the low piece then belongs to a neighbour of it
+        // the high piece by one instruction of its own, so that the low piece is
+        // the rest of that very value
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
-            const float y = w[j] * ratio, z = w[j + 1] * ratio;
-            const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(y, z));
+            const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(w[j], w[j + 1]));
             p[0][j] = h[0];
             p[0][j + 1] = h[1];
-            p[NP - 1][j] = (_Float16)(y - (float)h[0]);
-            p[NP - 1][j + 1] = (_Float16)(z - (float)h[1]);
+            p[NP - 1][j] = (_Float16)(w[j] - (float)h[0]);
+            p[NP - 1][j + 1] = (_Float16)(w[j + 1] - (float)h[1]);
         }
     }
+}
+
+// What rows see of the blocks from position `base` on, in 32 bits: a row's lo ..
+// hi there.
+__device__ __forceinline__ int32_t from(int64_t p, int64_t base)
+{
+    return (int32_t)max((int64_t)0, min(p - base, (int64_t)0x40000000));
 }
 
 // Row r of a tile of M pairs: its row of q and out, and its positions.
@@ -376,12 +389,11 @@ struct Row {
 template <uint32_t M> __device__ __forceinline__ Row row_of(const Problem &a, const Span &s, uint32_t head, uint32_t tile, uint32_t r)
 {
     Row w;
-    const uint64_t pair = (uint64_t)tile * M + r;
-    w.valid = pair < (uint64_t)s.n * a.n_rep;
-    const uint64_t i = w.valid ? pair / a.n_rep : 0;
+    const uint32_t pair = tile * M + r;
+    w.valid = pair < s.n * a.n_rep;
+    const uint32_t i = w.valid ? pair / a.n_rep : 0;
     w.row = s.row + i;
-    w.head = head * a.n_rep + (uint32_t)(pair - i * a.n_rep);
-    if (!w.valid) w.head = 0;
+    w.head = w.valid ? head * a.n_rep + (pair - i * a.n_rep) : 0;
     sight(a, s, s.pos + (int64_t)i, &w.lo, &w.hi);
     if (!w.valid) {                              // masks nothing, and is not stored
         w.lo = 0;
@@ -466,7 +478,8 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
         const uint8_t *vb = a.v.codes + (all + sh) * a.v.n_blocks * (kBlock * DP) + lane * 16u;
         const float *ks = a.v.scale + sh * a.v.n_blocks, *vs = a.v.scale + (all + sh) * a.v.n_blocks;
         const uint32_t last = it.t.blk0 + min(it.t.blocks, (c0 + nc) * kChunk);
-        uint32_t blk = it.t.blk0 + c0 * kChunk + wave;
+        const uint32_t blk0 = it.t.blk0 + c0 * kChunk;
+        uint32_t blk = blk0 + wave;
         uint4 k[NK], v[NV];
         float ksc = 0.f, vsc = 0.f;
         auto fetch = [&](uint32_t b) {
@@ -482,12 +495,13 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
         const Row row = row_of<kFewM>(a, it.s, it.head, it.tile, r);
         QFrag<DP, NP> q;
         load_q<DP, NP>(a, row.valid, row.row * a.q.ld_row + row.head * a.q.ld_head, g, q);
+        const int32_t lo = from(row.lo, (int64_t)blk0 * kBlock), hi = from(row.hi, (int64_t)blk0 * kBlock);
         State<DP> st;
         st.m = kLow;
         st.l = 0.f;
 #pragma unroll
         for (int i = 0; i < DP / 16; i++) st.o[i] = v4f{0.f, 0.f, 0.f, 0.f};
-        Ref ref{0.f};
+        Ref ref{0.f, 0.f};
         while (blk < last) {
             uint4 kc[NK], vc[NV];
 #pragma unroll
@@ -509,13 +523,25 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
                         acc[t] = mfma(y, q.h[n][2 * c + 1], acc[t]);
                     }
                 }
-            const float ratio = ratio_of<DP, 1>(vcs, ref, &st);
-            const int64_t b0 = (int64_t)blk * kBlock;
-            const bool masked = __any(row.lo > b0 || row.hi < b0 + (int64_t)kBlock);
-            const int32_t lo = row.lo > b0 ? (int32_t)min(row.lo - b0, (int64_t)kBlock) : 0;
-            const int32_t hi = row.hi > b0 ? (int32_t)min(row.hi - b0, (int64_t)kBlock) : 0;
+            float log, inv;
+            refer<DP, 1>(vcs, ref, &st);
+            ratio_of(vcs, ref, &log, &inv);
+            const int32_t off = (int32_t)(blk - blk0) * (int32_t)kBlock;
+            const float f = kcs * q.f;
+            const bool nan = vcs != vcs;
             h8 p[NP];
-            weigh<DP, NP>(acc, kcs * q.f, ratio, vcs, masked, lo, hi, g, st, p);
+            if (__any(lo > off || hi < off + (int32_t)kBlock) || nan) {
+                const uint32_t seen = seen_of(lo - off, hi - off, g);
+#pragma unroll
+                for (int j = 0; j < 8; j++) acc[j / 4][j % 4] = seen >> j & 1u ? acc[j / 4][j % 4] : -3.0e38f;
+                const float top = seen ? top_of(acc) * f : kLow;
+                if (__any(top > st.m + kLift)) lift(top, st);
+                weigh<DP, NP, true>(acc, f, log, inv, seen, nan, st, p);
+            } else {
+                const float top = top_of(acc) * f;
+                if (__any(top > st.m + kLift)) lift(top, st);
+                weigh<DP, NP, false>(acc, f, log, inv, 0, false, st, p);
+            }
 #pragma unroll
             for (int i = 0; i < DP / 32; i++) {
                 const h8 x = halves(vc[i].x, vc[i].y), y = halves(vc[i].z, vc[i].w);
@@ -616,7 +642,8 @@ template <int DP, int NP, int RT, int BT> __global__ void __launch_bounds__(256,
         const uint8_t *vb = a.v.codes + (all + sh) * a.v.n_blocks * (kBlock * DP);
         const float *ks = a.v.scale + sh * a.v.n_blocks, *vs = a.v.scale + (all + sh) * a.v.n_blocks;
         const uint32_t last = it.t.blk0 + min(it.t.blocks, (c0 + nc) * kChunk);
-        uint32_t blk = it.t.blk0 + c0 * kChunk;
+        const uint32_t blk0 = it.t.blk0 + c0 * kChunk;
+        uint32_t blk = blk0;
         uint4 code[BT][NU];
         float ksc[BT], vsc[BT], ksn[BT], vsn[BT];
         auto fetch = [&](uint32_t b) {
@@ -647,22 +674,21 @@ template <int DP, int NP, int RT, int BT> __global__ void __launch_bounds__(256,
         if (blk < last) fetch(blk);
         QFrag<DP, NP> q[RT];
         State<DP> st[RT];
-        int64_t lo[RT], hi[RT];
-        int64_t lo_all = 0, hi_all = INT64_MAX;
+        int32_t lo[RT], hi[RT], lo_all = 0, hi_all = 0x7FFFFFFF;
 #pragma unroll
         for (int t = 0; t < RT; t++) {
             const Row row = row_of<M>(a, it.s, it.head, it.tile, (wave * RT + t) * 16u + r);
             load_q<DP, NP>(a, row.valid, row.row * a.q.ld_row + row.head * a.q.ld_head, g, q[t]);
-            lo[t] = row.lo;
-            hi[t] = row.hi;
-            lo_all = max(lo_all, row.lo);
-            hi_all = min(hi_all, row.hi);
+            lo[t] = from(row.lo, (int64_t)blk0 * kBlock);
+            hi[t] = from(min(row.hi, (int64_t)last * kBlock), (int64_t)blk0 * kBlock);
+            lo_all = max(lo_all, lo[t]);
+            hi_all = min(hi_all, hi[t]);
             st[t].m = kLow;
             st[t].l = 0.f;
 #pragma unroll
             for (int i = 0; i < DP / 16; i++) st[t].o[i] = v4f{0.f, 0.f, 0.f, 0.f};
         }
-        Ref ref{0.f};
+        Ref ref{0.f, 0.f};
         uint32_t buf = 0;
         if (blk < last) put(0);
         __syncthreads();
@@ -674,42 +700,79 @@ template <int DP, int NP, int RT, int BT> __global__ void __launch_bounds__(256,
             }
             const bool more = blk + BT < last;
             if (more) fetch(blk + BT);
+            const h8 *const kf = stage + buf * kBuf + lane, *const vf = kf + kOne;
+            v4f acc[RT][BT][2];
 #pragma unroll
             for (int t = 0; t < BT; t++) {
-                const h8 *kf = stage + buf * kBuf + t * 2 * kOne + lane, *vf = kf + kOne;
-                v4f acc[RT][2];
 #pragma unroll
-                for (int x = 0; x < RT; x++) acc[x][0] = acc[x][1] = v4f{0.f, 0.f, 0.f, 0.f};
+                for (int x = 0; x < RT; x++) acc[x][t][0] = acc[x][t][1] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < DP / 32; c++)
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
-                        const h8 w = kf[(k * (DP / 32) + c) * 64];
+                        const h8 w = kf[t * 2 * kOne + (k * (DP / 32) + c) * 64];
 #pragma unroll
                         for (int x = 0; x < RT; x++)
 #pragma unroll
-                            for (int n = 0; n < NP; n++) acc[x][k] = mfma(w, q[x].h[n][c], acc[x][k]);
+                            for (int n = 0; n < NP; n++) acc[x][t][k] = mfma(w, q[x].h[n][c], acc[x][t][k]);
                     }
-                const float ratio = ratio_of<DP, RT>(vsc[t], ref, st);
-                const int64_t b0 = (int64_t)(blk + t) * kBlock;
-                const bool none = blk + t >= last;
-                const bool masked = __any(none || lo_all > b0 || hi_all < b0 + (int64_t)kBlock);
-                h8 p[RT][NP];
+            }
+            // all that may branch first: ratios, masks, references
+            float log[BT], inv[BT];
+            bool nan = false;
+            refer<DP, RT>(fmaxf(vsc[0], vsc[BT - 1]), ref, st);
 #pragma unroll
-                for (int x = 0; x < RT; x++) {
-                    const int32_t l = lo[x] > b0 ? (int32_t)min(lo[x] - b0, (int64_t)kBlock) : 0;
-                    const int32_t h = none ? 0 : hi[x] > b0 ? (int32_t)min(hi[x] - b0, (int64_t)kBlock) : 0;
-                    weigh<DP, NP>(acc[x], ksc[t] * q[x].f, ratio, vsc[t], masked, l, h, g, st[x], p[x]);
+            for (int t = 0; t < BT; t++) {
+                ratio_of(vsc[t], ref, &log[t], &inv[t]);
+                nan = nan || vsc[t] != vsc[t];
+            }
+            const int32_t off = (int32_t)(blk - blk0) * (int32_t)kBlock;
+            const bool some = __any(lo_all > off || hi_all < off + BT * (int32_t)kBlock) || nan;
+            uint32_t seen[RT][BT];
+            float top[RT];
+            bool past = false;
+#pragma unroll
+            for (int x = 0; x < RT; x++) {
+                top[x] = kLow;
+#pragma unroll
+                for (int t = 0; t < BT; t++) {
+                    seen[x][t] = 0xFFu;
+                    if (some) {
+                        const int32_t o = off + t * (int32_t)kBlock;
+                        seen[x][t] = seen_of(lo[x] - o, hi[x] - o, g);
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            acc[x][t][j / 4][j % 4] = seen[x][t] >> j & 1u ? acc[x][t][j / 4][j % 4] : -3.0e38f;
+                    }
+                    const float m = top_of(acc[x][t]) * (ksc[t] * q[x].f);
+                    top[x] = fmaxf(top[x], seen[x][t] ? m : kLow);
                 }
+                past = past || top[x] > st[x].m + kLift;
+            }
+            if (__any(past)) {
 #pragma unroll
-                for (int i = 0; i < DP / 16; i++) {
-                    const h8 w = vf[i * 64];
+                for (int x = 0; x < RT; x++) lift(top[x], st[x]);
+            }
+            auto rest = [&](auto SOME) {
+#pragma unroll
+                for (int t = 0; t < BT; t++) {
+                    h8 p[RT][NP];
 #pragma unroll
                     for (int x = 0; x < RT; x++)
+                        weigh<DP, NP, decltype(SOME)::value>(acc[x][t], ksc[t] * q[x].f, log[t], inv[t], seen[x][t],
+                                                             vsc[t] != vsc[t], st[x], p[x]);
 #pragma unroll
-                        for (int n = 0; n < NP; n++) st[x].o[i] = mfma(w, p[x][n], st[x].o[i]);
+                    for (int i = 0; i < DP / 16; i++) {
+                        const h8 w = vf[t * 2 * kOne + i * 64];
+#pragma unroll
+                        for (int x = 0; x < RT; x++)
+#pragma unroll
+                            for (int n = 0; n < NP; n++) st[x].o[i] = mfma(w, p[x][n], st[x].o[i]);
+                    }
                 }
-            }
+            };
+            if (some) rest(std::true_type{});
+            else rest(std::false_type{});
             if (more) put(buf ^ 1u);
             buf ^= 1u;
             __syncthreads();
