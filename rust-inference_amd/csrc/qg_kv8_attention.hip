@@ -20,12 +20,12 @@
 //     high in f16's range as it can, for the low pieces' bits.
 //   * vs goes into p as a ratio to a running reference scale that moves only when
 //     the ratio leaves 2^-6 .. 2, so the accumulators are not touched per block.
-//   * masked positions: p = 0 whatever their codes; a NaN scale (non-finite block)
-//     reaches the rows that see a position of the block.
+//   * masked positions: a score of -inf, p = 0 whatever their codes; a block with a
+//     NaN scale reaches the rows that see a position of it.
 //
 // Rows are (token, query head) pairs of one kv head: pair r of a sequence is token
 // r / n_rep, head r % n_rep (the callers keep n_rows * n_rep below 2^31).  Tiles of kM pairs of one sequence and kv head are the
-// items; an item's work is its visible blocks in chunks of kChunk.  All items'
+// items; an item's work is its visible blocks in chunks of a few.  All items'
 // chunks, end to end, are dealt out evenly to the workgroups (about two per
 // compute unit) whatever the sequences' lengths; a workgroup's share may end
 // inside an item, then the parts' (m, sum, unnormalised output) go to the
@@ -34,7 +34,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <type_traits>
 
 namespace qg8 {
 namespace {
@@ -43,7 +42,6 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kChunk = 4;                // blocks
 constexpr float kBias = 12.f, kLift = 2.f;   // 2^(12 + 2) times a ratio of 2: f16's largest power
 constexpr float kLow = -3.0e38f;              // below any score
 constexpr uint32_t kNone = 0xFFFFFFFFu;
@@ -70,11 +68,18 @@ struct Problem {
     View v;
     Batch b;
     Rows q, out;
-    uint32_t n_rep, window;
+    uint32_t n_rep, rep_mul, rep_shift;    // x / n_rep = (mulhi(x, rep_mul) + x) >> rep_shift for x < 2^31
+    uint32_t window;
+    uint32_t chunk;                        // blocks that are dealt out together
     float scale2;      // |scale| log2(e)
     float sign;
     Work w;
 };
+
+__device__ __forceinline__ uint32_t over_rep(const Problem &a, uint32_t x)
+{
+    return (__umulhi(x, a.rep_mul) + x) >> a.rep_shift;
+}
 
 // First position and one past the last that the token at position p sees.
 __device__ __forceinline__ void sight(const Problem &a, const Span &s, int64_t p, int64_t *lo, int64_t *hi)
@@ -93,8 +98,8 @@ template <uint32_t M> __device__ __forceinline__ Tile tile_of(const Problem &a, 
 {
     const uint32_t r0 = t * M, r1 = min(r0 + M, s.n * a.n_rep) - 1;
     int64_t lo, hi, x, y;
-    sight(a, s, s.pos + (int64_t)(r0 / a.n_rep), &lo, &x);
-    sight(a, s, s.pos + (int64_t)(r1 / a.n_rep), &y, &hi);
+    sight(a, s, s.pos + (int64_t)over_rep(a, r0), &lo, &x);
+    sight(a, s, s.pos + (int64_t)over_rep(a, r1), &y, &hi);
     Tile k;
     k.blk0 = 0;
     k.blocks = 0;
@@ -102,27 +107,45 @@ template <uint32_t M> __device__ __forceinline__ Tile tile_of(const Problem &a, 
         k.blk0 = (uint32_t)(lo / kBlock);
         k.blocks = (uint32_t)((hi - 1) / kBlock) - k.blk0 + 1;
     }
-    k.chunks = max(1u, (k.blocks + kChunk - 1) / kChunk);
+    k.chunks = max(1u, (k.blocks + a.chunk - 1) / a.chunk);
     return k;
 }
 
+// Sums over the lanes up to each (DPP: shifts within the rows of 16, then the
+// rows' last lanes to the rows behind them), and the last one's.
+template <int CTRL, int ROWS = 0xF> __device__ __forceinline__ uint32_t dpp0(uint32_t v)
+{
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ uint32_t scan64(uint32_t v)
+{
+    v += dpp0<0x111>(v);
+    v += dpp0<0x112>(v);
+    v += dpp0<0x114>(v);
+    v += dpp0<0x118>(v);
+    v += dpp0<0x142, 0xA>(v);
+    v += dpp0<0x143, 0xC>(v);
+    return v;
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, uint32_t l)
+{
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)l);
+}
+
 // Chunks of all tiles of a sequence (one kv head), by the whole wave.
-template <uint32_t M> __device__ uint64_t seq_chunks(const Problem &a, const Span &s)
+template <uint32_t M> __device__ uint32_t seq_chunks(const Problem &a, const Span &s)
 {
     const uint32_t n = tiles_of<M>(a, s), lane = threadIdx.x & 63u;
-    uint64_t c = 0;
+    uint32_t c = 0;
     for (uint32_t t = lane; t < n; t += 64) c += tile_of<M>(a, s, t).chunks;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) c += __shfl_xor((unsigned long long)c, o, 64);
-    return c;
+    return lane_of(scan64(c), 63);
 }
 
 // Chunks of 64 sequences from s0 on, a sequence per lane, all kv heads.
-template <uint32_t M> __device__ uint64_t lane_chunks(const Problem &a, uint32_t s0)
+template <uint32_t M> __device__ uint32_t lane_chunks(const Problem &a, uint32_t s0)
 {
     const uint32_t lane = threadIdx.x & 63u, s = s0 + lane;
-    uint32_t n = 0;
-    uint64_t c = 0;
+    uint32_t n = 0, c = 0;
     if (s < a.v.n_seqs) {
         const Span p = span_of(a.b, s);
         n = tiles_of<M>(a, p);
@@ -132,76 +155,63 @@ template <uint32_t M> __device__ uint64_t lane_chunks(const Problem &a, uint32_t
     while (many) {
         const uint32_t l = (uint32_t)__ffsll((unsigned long long)many) - 1;
         many &= many - 1;
-        const uint64_t t = seq_chunks<M>(a, span_of(a.b, s0 + l));
+        const uint32_t t = seq_chunks<M>(a, span_of(a.b, s0 + l));
         if (lane == l) c = t;
     }
     return c * a.v.n_heads;
 }
 
-__device__ __forceinline__ uint64_t scan64(uint64_t c)
-{
-    const uint32_t lane = threadIdx.x & 63u;
-#pragma unroll
-    for (uint32_t o = 1; o < 64; o <<= 1) {
-        const uint64_t up = __shfl_up((unsigned long long)c, o, 64);
-        if (lane >= o) c += up;
-    }
-    return c;
-}
-
 struct Item {
     uint32_t seq, head, tile;
-    uint64_t start;                     // chunk the item begins with
+    uint32_t start;                     // chunk the item begins with
     Tile t;
     Span s;
 };
 
 // All sequences' chunks; `first` keeps the running sums of the first 64.
-template <uint32_t M> __device__ uint64_t all_chunks(const Problem &a, uint64_t *first)
+template <uint32_t M> __device__ uint32_t all_chunks(const Problem &a, uint32_t *first)
 {
-    uint64_t total = 0;
+    uint32_t total = 0;
     for (uint32_t s0 = 0; s0 < a.v.n_seqs; s0 += 64) {
-        const uint64_t c = scan64(lane_chunks<M>(a, s0));
+        const uint32_t c = scan64(lane_chunks<M>(a, s0));
         if (s0 == 0) *first = c;
-        total += __shfl((unsigned long long)c, 63, 64);
+        total += lane_of(c, 63);
     }
     return total;
 }
 
 // The item that holds chunk `at` (less than the total).
-template <uint32_t M> __device__ Item find(const Problem &a, uint64_t at, uint64_t first)
+template <uint32_t M> __device__ Item find(const Problem &a, uint32_t at, uint32_t first)
 {
     const uint32_t lane = threadIdx.x & 63u;
     Item it{};
-    uint64_t before = 0;
+    uint32_t before = 0;
     for (uint32_t s0 = 0; s0 < a.v.n_seqs; s0 += 64) {
-        const uint64_t c = s0 == 0 ? first : scan64(lane_chunks<M>(a, s0));
+        const uint32_t c = s0 == 0 ? first : scan64(lane_chunks<M>(a, s0));
         const uint64_t past = __ballot(before + c > at);
         if (!past) {
-            before += __shfl((unsigned long long)c, 63, 64);
+            before += lane_of(c, 63);
             continue;
         }
         const uint32_t l = (uint32_t)__ffsll((unsigned long long)past) - 1;
-        const uint64_t up_to = __shfl((unsigned long long)c, (int)l, 64);
-        const uint64_t below = l ? __shfl((unsigned long long)c, (int)l - 1, 64) : 0ull;
+        const uint32_t up_to = lane_of(c, l), below = l ? lane_of(c, l - 1) : 0u;
         it.seq = s0 + l;
         it.s = span_of(a.b, it.seq);
         before += below;
-        const uint64_t per_head = (up_to - below) / a.v.n_heads;
-        it.head = (uint32_t)((at - before) / per_head);
+        const uint32_t per_head = (up_to - below) / a.v.n_heads;
+        it.head = (at - before) / per_head;
         before += it.head * per_head;
         const uint32_t n = tiles_of<M>(a, it.s);
         for (uint32_t t0 = 0; t0 < n; t0 += 64) {
-            const uint32_t w = t0 + lane < n ? tile_of<M>(a, it.s, t0 + lane).chunks : 0u;
-            const uint64_t d = n == 1 ? (uint64_t)__shfl((int)w, 0, 64) : scan64(w);
+            const uint32_t d = n == 1 ? per_head : scan64(t0 + lane < n ? tile_of<M>(a, it.s, t0 + lane).chunks : 0u);
             const uint64_t in = __ballot(before + d > at);
             if (!in) {
-                before += __shfl((unsigned long long)d, 63, 64);
+                before += lane_of(d, 63);
                 continue;
             }
             const uint32_t k = (uint32_t)__ffsll((unsigned long long)in) - 1;
             it.tile = t0 + k;
-            it.start = before + (k ? __shfl((unsigned long long)d, (int)k - 1, 64) : 0ull);
+            it.start = before + (k ? lane_of(d, k - 1) : 0u);
             it.t = tile_of<M>(a, it.s, it.tile);
             return it;
         }
@@ -299,7 +309,7 @@ template <int DP, int NT> __device__ __forceinline__ void refer(float vs, Ref &r
 }
 
 // vs / ref as a power of two, and inverted.  A scale of 0 (all codes zero) or NaN
-// (see weigh) counts as 1; one that is nothing beside the reference as 2^-100,
+// (see mask) counts as 1; one that is nothing beside the reference as 2^-100,
 // which f16 does not hold either.
 __device__ __forceinline__ void ratio_of(float vs, const Ref &r, float *log, float *inv)
 {
@@ -321,10 +331,13 @@ __device__ __forceinline__ uint32_t seen_of(int32_t lo, int32_t hi, uint32_t g)
     return s;
 }
 
-// Largest of a lane's eight scores.
+// Largest of a lane's eight scores; NaN if one is (the row is then NaN whatever
+// its reference).  maximum, not fmaxf: one instruction for three values, which
+// need not be made quiet first.
 __device__ __forceinline__ float top_of(const v4f *x)
 {
-    return fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+    auto top = [](float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); };
+    return top(top(x[0][0], x[0][1], x[0][2]), top(x[0][3], x[1][0], x[1][1]), __builtin_elementwise_maximum(x[1][2], x[1][3]));
 }
 
 // Moves the rows' references up where `top` (a lane's largest score) is past them.
@@ -339,36 +352,44 @@ template <int DP> __device__ __forceinline__ void lift(float top, State<DP> &st)
     for (int i = 0; i < DP / 16; i++) st.o[i] *= k;
 }
 
-// A block's scores x into p, kBias above the row's reference, and its f16
-// pieces.  log, inv: the block's ratio (2^log, 1 / it).  SOME: positions outside
-// `seen` weigh nothing, and where `nan` is set the others weigh NaN.
-template <int DP, int NP, bool SOME>
-__device__ __forceinline__ void weigh(const v4f *x, float f, float log, float inv, uint32_t seen, bool nan, State<DP> &st, h8 *p)
+// The factor of a row's scores of a block; never 0, so that a masked score of
+// -inf stays one (NaN for a row of q that is not finite).
+__device__ __forceinline__ float factor(float ks, float f)
 {
-    const float c = kBias - st.m + log;
-    float w[8];
+    const float x = ks * f;
+    return x < 0x1p-126f ? 0x1p-126f : x;
+}
+
+// Scores of positions outside lo .. hi of a block to -inf.  A block whose scale
+// is not a number makes the sum of every row that sees of it NaN, and is then as
+// if masked for all (its scales become 1).
+__device__ __forceinline__ void mask(v4f *x, int32_t lo, int32_t hi, uint32_t g, bool nan, float &l)
+{
+    const uint32_t seen = seen_of(lo, hi, g);
 #pragma unroll
-    for (int j = 0; j < 8; j++) w[j] = exp2_(__builtin_fmaf(x[j / 4][j % 4], f, c));
-    if (SOME) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) w[j] = seen >> j & 1u ? (nan ? __uint_as_float(0x7FC00000u) : w[j]) : 0.f;
-    }
-    st.l = __builtin_fmaf(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])), inv, st.l);
+    for (int j = 0; j < 8; j++) x[j / 4][j % 4] = !nan && (seen >> j & 1u) ? x[j / 4][j % 4] : -INFINITY;
+    if (nan && seen) l = __uint_as_float(0x7FC00000u);
+}
+
+// Weights of a block's scores: w_j = 2^(f x_j + c), kBias above the row's reference
+// (c = kBias - m + log2 of the block's value ratio), as f16 pieces p.  Two at a
+// time, so that they can be spread between products.
+template <int NP> __device__ __forceinline__ float weigh2(float x, float y, float f, float c, int j, h8 *p)
+{
+    const float a = exp2_(__builtin_fmaf(x, f, c)), b = exp2_(__builtin_fmaf(y, f, c));
     if (NP == 1) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) p[0][j] = (_Float16)w[j];
+        p[0][j] = (_Float16)a;
+        p[0][j + 1] = (_Float16)b;
     } else {
         // the high piece by one instruction of its own, so that the low piece is
         // the rest of that very value
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(w[j], w[j + 1]));
-            p[0][j] = h[0];
-            p[0][j + 1] = h[1];
-            p[NP - 1][j] = (_Float16)(w[j] - (float)h[0]);
-            p[NP - 1][j + 1] = (_Float16)(w[j + 1] - (float)h[1]);
-        }
+        const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
+        p[0][j] = h[0];
+        p[0][j + 1] = h[1];
+        p[NP - 1][j] = (_Float16)(a - (float)h[0]);
+        p[NP - 1][j + 1] = (_Float16)(b - (float)h[1]);
     }
+    return a + b;
 }
 
 // What rows see of the blocks from position `base` on, in 32 bits: a row's lo ..
@@ -391,7 +412,7 @@ template <uint32_t M> __device__ __forceinline__ Row row_of(const Problem &a, co
     Row w;
     const uint32_t pair = tile * M + r;
     w.valid = pair < s.n * a.n_rep;
-    const uint32_t i = w.valid ? pair / a.n_rep : 0;
+    const uint32_t i = w.valid ? over_rep(a, pair) : 0;
     w.row = s.row + i;
     w.head = w.valid ? head * a.n_rep + (pair - i * a.n_rep) : 0;
     sight(a, s, s.pos + (int64_t)i, &w.lo, &w.hi);
@@ -420,14 +441,14 @@ __device__ __forceinline__ void store_row(const Rows &o, uint64_t at, uint32_t d
     }
 }
 
-template <uint32_t M> __device__ __forceinline__ void put_split(const Problem &a, uint32_t wg, const Item *it, uint64_t per)
+template <uint32_t M> __device__ __forceinline__ void put_split(const Problem &a, uint32_t wg, const Item *it, uint32_t per)
 {
     if (threadIdx.x) return;
     Split s{};
     s.first = kNone;
     if (it) {
-        s.first = (uint32_t)(it->start / per);
-        s.last = (uint32_t)((it->start + it->t.chunks - 1) / per);
+        s.first = it->start / per;
+        s.last = (it->start + it->t.chunks - 1) / per;
         s.seq = it->seq;
         s.head = it->head;
         s.tile = it->tile;
@@ -455,11 +476,11 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
     __shared__ float so[4][16][LD], sm[4][16], sl[4][16];
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
     const uint32_t wg = place_of(blockIdx.x, gridDim.x);
-    uint64_t first;
-    const uint64_t total = all_chunks<kFewM>(a, &first);
-    const uint64_t per = (total + gridDim.x - 1) / gridDim.x;
-    uint64_t at = wg * per;
-    const uint64_t end = min(at + per, total);
+    uint32_t first;
+    const uint32_t total = all_chunks<kFewM>(a, &first);
+    const uint32_t per = (total + gridDim.x - 1) / gridDim.x;
+    uint32_t at = wg * per;
+    const uint32_t end = min(at + per, total);
     if (at >= end) {
         put_split<kFewM>(a, wg, nullptr, per);
         return;
@@ -468,7 +489,7 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
     const uint64_t all = (uint64_t)a.v.n_seqs * a.v.n_heads;
     while (at < end) {
         const Item it = find<kFewM>(a, at, first);
-        const uint32_t c0 = (uint32_t)(at - it.start), nc = (uint32_t)min((uint64_t)(it.t.chunks - c0), end - at);
+        const uint32_t c0 = at - it.start, nc = min(it.t.chunks - c0, end - at);
         if (!begun) {
             put_split<kFewM>(a, wg, c0 ? &it : nullptr, per);
             begun = true;
@@ -477,8 +498,8 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
         const uint8_t *kb = a.v.codes + sh * a.v.n_blocks * (kBlock * DP) + lane * 16u;
         const uint8_t *vb = a.v.codes + (all + sh) * a.v.n_blocks * (kBlock * DP) + lane * 16u;
         const float *ks = a.v.scale + sh * a.v.n_blocks, *vs = a.v.scale + (all + sh) * a.v.n_blocks;
-        const uint32_t last = it.t.blk0 + min(it.t.blocks, (c0 + nc) * kChunk);
-        const uint32_t blk0 = it.t.blk0 + c0 * kChunk;
+        const uint32_t last = it.t.blk0 + min(it.t.blocks, (c0 + nc) * a.chunk);
+        const uint32_t blk0 = it.t.blk0 + c0 * a.chunk;
         uint32_t blk = blk0 + wave;
         uint4 k[NK], v[NV];
         float ksc = 0.f, vsc = 0.f;
@@ -527,21 +548,17 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
             refer<DP, 1>(vcs, ref, &st);
             ratio_of(vcs, ref, &log, &inv);
             const int32_t off = (int32_t)(blk - blk0) * (int32_t)kBlock;
-            const float f = kcs * q.f;
-            const bool nan = vcs != vcs;
+            const bool nan = kcs != kcs || vcs != vcs;
+            const float f = factor(nan ? 1.f : kcs, q.f);
+            if (__any(lo > off || hi < off + (int32_t)kBlock) || nan) mask(acc, lo - off, hi - off, g, nan, st.l);
+            const float top = top_of(acc) * f;
+            if (__any(top > st.m + kLift)) lift(top, st);
             h8 p[NP];
-            if (__any(lo > off || hi < off + (int32_t)kBlock) || nan) {
-                const uint32_t seen = seen_of(lo - off, hi - off, g);
+            const float c = kBias - st.m + log;
+            float sum = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; j++) acc[j / 4][j % 4] = seen >> j & 1u ? acc[j / 4][j % 4] : -3.0e38f;
-                const float top = seen ? top_of(acc) * f : kLow;
-                if (__any(top > st.m + kLift)) lift(top, st);
-                weigh<DP, NP, true>(acc, f, log, inv, seen, nan, st, p);
-            } else {
-                const float top = top_of(acc) * f;
-                if (__any(top > st.m + kLift)) lift(top, st);
-                weigh<DP, NP, false>(acc, f, log, inv, 0, false, st, p);
-            }
+            for (int j = 0; j < 8; j += 2) sum += weigh2<NP>(acc[j / 4][j % 4], acc[j / 4][j % 4 + 1], f, c, j, p);
+            st.l = __builtin_fmaf(sum, inv, st.l);
 #pragma unroll
             for (int i = 0; i < DP / 32; i++) {
                 const h8 x = halves(vc[i].x, vc[i].y), y = halves(vc[i].z, vc[i].w);
@@ -607,23 +624,26 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
 }
 
 // Many rows: tiles of 64 RT pairs, 16 RT a wave.  The workgroup's waves share
-// an item's blocks: BT at a time their codes are loaded into registers (a step
-// ahead), turned into f16 once and put into one of two LDS buffers in the order of
-// the operands, from where every wave feeds its products (a K or V operand is
-// read once for RT of them).
-template <int DP, int NP, int RT, int BT> __global__ void __launch_bounds__(256, 2) many_k(Problem a)
+// an item's blocks: a block's codes are loaded into registers three blocks ahead,
+// turned into f16 once and put into a ring of three in LDS in the order of the
+// operands, from where every wave feeds its products (an operand is read once
+// for RT tiles of rows).  Within a wave the matrix cores and the vector units
+// work at the same time: the scores of block j + 1 while block j's are turned
+// into weights, the outputs of block j while the codes of block j + 2 are turned
+// into f16.
+template <int DP, int NP, int RT> __global__ void __launch_bounds__(256, 2) many_k(Problem a)
 {
     constexpr uint32_t M = 64 * RT;
     constexpr int NU = DP / 64;                           // 16-byte units of codes a thread stages per block
-    extern __shared__ __attribute__((aligned(16))) h8 stage[];        // [2][BT][keys, values][DP / 32 * 2][64]
-    constexpr uint32_t kOne = DP * 4, kBuf = BT * 2 * kOne;           // operands of 16 bytes: keys or values of a block, a buffer
+    extern __shared__ __attribute__((aligned(16))) h8 stage[];        // [3][keys, values][DP / 32 * 2][64]
+    constexpr uint32_t kOne = DP * 4;                                 // operands of 16 bytes: keys or values of a block
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
     const uint32_t wg = place_of(blockIdx.x, gridDim.x);
-    uint64_t first;
-    const uint64_t total = all_chunks<M>(a, &first);
-    const uint64_t per = (total + gridDim.x - 1) / gridDim.x;
-    uint64_t at = wg * per;
-    const uint64_t end = min(at + per, total);
+    uint32_t first;
+    const uint32_t total = all_chunks<M>(a, &first);
+    const uint32_t per = (total + gridDim.x - 1) / gridDim.x;
+    uint32_t at = wg * per;
+    const uint32_t end = min(at + per, total);
     if (at >= end) {
         put_split<M>(a, wg, nullptr, per);
         return;
@@ -632,46 +652,35 @@ template <int DP, int NP, int RT, int BT> __global__ void __launch_bounds__(256,
     const uint64_t all = (uint64_t)a.v.n_seqs * a.v.n_heads;
     while (at < end) {
         const Item it = find<M>(a, at, first);
-        const uint32_t c0 = (uint32_t)(at - it.start), nc = (uint32_t)min((uint64_t)(it.t.chunks - c0), end - at);
+        const uint32_t c0 = at - it.start, nc = min(it.t.chunks - c0, end - at);
         if (!begun) {
             put_split<M>(a, wg, c0 ? &it : nullptr, per);
             begun = true;
         }
         const uint64_t sh = (uint64_t)it.seq * a.v.n_heads + it.head;
-        const uint8_t *kb = a.v.codes + sh * a.v.n_blocks * (kBlock * DP);
-        const uint8_t *vb = a.v.codes + (all + sh) * a.v.n_blocks * (kBlock * DP);
-        const float *ks = a.v.scale + sh * a.v.n_blocks, *vs = a.v.scale + (all + sh) * a.v.n_blocks;
-        const uint32_t last = it.t.blk0 + min(it.t.blocks, (c0 + nc) * kChunk);
-        const uint32_t blk0 = it.t.blk0 + c0 * kChunk;
-        uint32_t blk = blk0;
-        uint4 code[BT][NU];
-        float ksc[BT], vsc[BT], ksn[BT], vsn[BT];
+        // the part's first block; n of them (0: an item that sees nothing)
+        const uint32_t blk0 = it.t.blk0 + c0 * a.chunk;
+        const uint32_t n = it.t.blk0 + min(it.t.blocks, (c0 + nc) * a.chunk) - blk0;
+        const uint8_t *kb = a.v.codes + (sh * a.v.n_blocks + blk0) * (kBlock * DP);
+        const uint8_t *vb = a.v.codes + ((all + sh) * a.v.n_blocks + blk0) * (kBlock * DP);
+        const float *ks = a.v.scale + sh * a.v.n_blocks + blk0, *vs = a.v.scale + (all + sh) * a.v.n_blocks + blk0;
+        uint4 code[NU];
+        // the blocks' codes; the last one's again behind it
         auto fetch = [&](uint32_t b) {
+            const uint64_t off = (uint64_t)min(b, n - 1) * (kBlock * DP);
 #pragma unroll
-            for (int t = 0; t < BT; t++) {
-                const uint32_t bt = min(b + t, last - 1);
-                const uint64_t off = (uint64_t)bt * (kBlock * DP);
-#pragma unroll
-                for (int i = 0; i < NU; i++) {
-                    const uint32_t u = threadIdx.x + 256u * i;
-                    code[t][i] = *(const uint4 *)(u < 2 * DP ? kb + off + u * 16u : vb + off + (u - 2 * DP) * 16u);
-                }
-                ksn[t] = ks[bt];
-                vsn[t] = vs[bt];
+            for (int i = 0; i < NU; i++) {
+                const uint32_t u = threadIdx.x + 256u * i;
+                code[i] = *(const uint4 *)(u < 2 * DP ? kb + off + u * 16u : vb + off + (u - 2 * DP) * 16u);
             }
         };
-        auto put = [&](uint32_t buf) {
-#pragma unroll
-            for (int t = 0; t < BT; t++)
-#pragma unroll
-                for (int i = 0; i < NU; i++) {
-                    const uint32_t u = threadIdx.x + 256u * i;
-                    h8 *to = stage + buf * kBuf + t * 2 * kOne + (u >> 6) * 128u + lane;
-                    to[0] = halves(code[t][i].x, code[t][i].y);
-                    to[64] = halves(code[t][i].z, code[t][i].w);
-                }
+        auto put = [&](uint32_t slot, int half) {         // half: of 2 NU
+            const uint32_t u = threadIdx.x + 256u * (half / 2);
+            h8 *to = stage + slot * 2 * kOne + (u >> 6) * 128u + lane + half % 2 * 64;
+            const uint4 w = code[half / 2];
+            *to = half % 2 ? halves(w.z, w.w) : halves(w.x, w.y);
         };
-        if (blk < last) fetch(blk);
+        if (n) fetch(0);
         QFrag<DP, NP> q[RT];
         State<DP> st[RT];
         int32_t lo[RT], hi[RT], lo_all = 0, hi_all = 0x7FFFFFFF;
@@ -680,7 +689,7 @@ template <int DP, int NP, int RT, int BT> __global__ void __launch_bounds__(256,
             const Row row = row_of<M>(a, it.s, it.head, it.tile, (wave * RT + t) * 16u + r);
             load_q<DP, NP>(a, row.valid, row.row * a.q.ld_row + row.head * a.q.ld_head, g, q[t]);
             lo[t] = from(row.lo, (int64_t)blk0 * kBlock);
-            hi[t] = from(min(row.hi, (int64_t)last * kBlock), (int64_t)blk0 * kBlock);
+            hi[t] = from(row.hi, (int64_t)blk0 * kBlock);
             lo_all = max(lo_all, lo[t]);
             hi_all = min(hi_all, hi[t]);
             st[t].m = kLow;
@@ -689,93 +698,124 @@ template <int DP, int NP, int RT, int BT> __global__ void __launch_bounds__(256,
             for (int i = 0; i < DP / 16; i++) st[t].o[i] = v4f{0.f, 0.f, 0.f, 0.f};
         }
         Ref ref{0.f, 0.f};
-        uint32_t buf = 0;
-        if (blk < last) put(0);
-        __syncthreads();
-        for (; blk < last; blk += BT) {
+        // S^T of the block in `slot`
+        auto scores = [&](uint32_t slot, v4f (&x)[RT][2]) {
+            const h8 *kf = stage + slot * 2 * kOne + lane;
 #pragma unroll
-            for (int t = 0; t < BT; t++) {
-                ksc[t] = ksn[t];
-                vsc[t] = vsn[t];
+            for (int t = 0; t < RT; t++) x[t][0] = x[t][1] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < DP / 32; c++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const h8 w = kf[(k * (DP / 32) + c) * 64];
+#pragma unroll
+                    for (int t = 0; t < RT; t++)
+#pragma unroll
+                        for (int i = 0; i < NP; i++) x[t][k] = mfma(w, q[t].h[i][c], x[t][k]);
+                }
+        };
+        float ksn = 0.f, vsn = 0.f;
+        // block j, its scores in x; the next one's into y.  slot: j % 3
+        auto block = [&](uint32_t j, uint32_t slot, v4f (&x)[RT][2], v4f (&y)[RT][2]) {
+            const float ksc = ksn, vsc = vsn;
+            const uint32_t next = min(j + 1, n - 1), s1 = slot == 2 ? 0u : slot + 1, s2 = slot == 0 ? 2u : slot - 1;
+            ksn = ks[next];
+            vsn = vs[next];
+            constexpr int kOps = DP / 16, kAhead = 4;     // operands of keys, and of values; in flight
+            const h8 *kf = stage + s1 * 2 * kOne + lane, *vf = stage + slot * 2 * kOne + kOne + lane;
+            h8 ops[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) ops[i] = kf[i * 64];
+            // what may branch first: the value scale's reference, masks, the rows' references
+            refer<DP, RT>(vsc, ref, st);
+            float log, inv;
+            ratio_of(vsc, ref, &log, &inv);
+            const bool nan = ksc != ksc || vsc != vsc;
+            const int32_t off = (int32_t)(j * kBlock);
+            if (__any(lo_all > off || hi_all < off + (int32_t)kBlock) || nan) {
+#pragma unroll
+                for (int t = 0; t < RT; t++) mask(x[t], lo[t] - off, hi[t] - off, g, nan, st[t].l);
             }
-            const bool more = blk + BT < last;
-            if (more) fetch(blk + BT);
-            const h8 *const kf = stage + buf * kBuf + lane, *const vf = kf + kOne;
-            v4f acc[RT][BT][2];
-#pragma unroll
-            for (int t = 0; t < BT; t++) {
-#pragma unroll
-                for (int x = 0; x < RT; x++) acc[x][t][0] = acc[x][t][1] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < DP / 32; c++)
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const h8 w = kf[t * 2 * kOne + (k * (DP / 32) + c) * 64];
-#pragma unroll
-                        for (int x = 0; x < RT; x++)
-#pragma unroll
-                            for (int n = 0; n < NP; n++) acc[x][t][k] = mfma(w, q[x].h[n][c], acc[x][t][k]);
-                    }
-            }
-            // all that may branch first: ratios, masks, references
-            float log[BT], inv[BT];
-            bool nan = false;
-            refer<DP, RT>(fmaxf(vsc[0], vsc[BT - 1]), ref, st);
-#pragma unroll
-            for (int t = 0; t < BT; t++) {
-                ratio_of(vsc[t], ref, &log[t], &inv[t]);
-                nan = nan || vsc[t] != vsc[t];
-            }
-            const int32_t off = (int32_t)(blk - blk0) * (int32_t)kBlock;
-            const bool some = __any(lo_all > off || hi_all < off + BT * (int32_t)kBlock) || nan;
-            uint32_t seen[RT][BT];
-            float top[RT];
+            float f[RT], top[RT];
             bool past = false;
 #pragma unroll
-            for (int x = 0; x < RT; x++) {
-                top[x] = kLow;
-#pragma unroll
-                for (int t = 0; t < BT; t++) {
-                    seen[x][t] = 0xFFu;
-                    if (some) {
-                        const int32_t o = off + t * (int32_t)kBlock;
-                        seen[x][t] = seen_of(lo[x] - o, hi[x] - o, g);
-#pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            acc[x][t][j / 4][j % 4] = seen[x][t] >> j & 1u ? acc[x][t][j / 4][j % 4] : -3.0e38f;
-                    }
-                    const float m = top_of(acc[x][t]) * (ksc[t] * q[x].f);
-                    top[x] = fmaxf(top[x], seen[x][t] ? m : kLow);
-                }
-                past = past || top[x] > st[x].m + kLift;
+            for (int t = 0; t < RT; t++) {
+                f[t] = factor(nan ? 1.f : ksc, q[t].f);
+                top[t] = top_of(x[t]) * f[t];
+                past = past || top[t] > st[t].m + kLift;
             }
             if (__any(past)) {
 #pragma unroll
-                for (int x = 0; x < RT; x++) lift(top[x], st[x]);
+                for (int t = 0; t < RT; t++) lift(top[t], st[t]);
             }
-            auto rest = [&](auto SOME) {
+            // operand by operand: its products, the read of the one kAhead behind it,
+            // and a share of the vector work (the order is held by barriers to the
+            // scheduler, which would put each part in one piece and wait for every
+            // read)
+            h8 p[RT][NP];
+            float c[RT], sum[RT];
 #pragma unroll
-                for (int t = 0; t < BT; t++) {
-                    h8 p[RT][NP];
+            for (int t = 0; t < RT; t++) {
+                c[t] = kBias - st[t].m + log;
+                sum[t] = 0.f;
+                y[t][0] = y[t][1] = v4f{0.f, 0.f, 0.f, 0.f};
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int x = 0; x < RT; x++)
-                        weigh<DP, NP, decltype(SOME)::value>(acc[x][t], ksc[t] * q[x].f, log[t], inv[t], seen[x][t],
-                                                             vsc[t] != vsc[t], st[x], p[x]);
+            for (int i = 0; i < kOps; i++) {
+                const h8 w = ops[i % kAhead];
+                if (i + kAhead < kOps) ops[i % kAhead] = kf[(i + kAhead) * 64];
+                else if (i + kAhead < 2 * kOps) ops[i % kAhead] = vf[(i + kAhead - kOps) * 64];
 #pragma unroll
-                    for (int i = 0; i < DP / 16; i++) {
-                        const h8 w = vf[t * 2 * kOne + i * 64];
+                for (int t = 0; t < RT; t++)
 #pragma unroll
-                        for (int x = 0; x < RT; x++)
+                    for (int k = 0; k < NP; k++)
+                        y[t][i / (kOps / 2)] = mfma(w, q[t].h[k][i % (kOps / 2)], y[t][i / (kOps / 2)]);
 #pragma unroll
-                            for (int n = 0; n < NP; n++) st[x].o[i] = mfma(w, p[x][n], st[x].o[i]);
-                    }
-                }
-            };
-            if (some) rest(std::true_type{});
-            else rest(std::false_type{});
-            if (more) put(buf ^ 1u);
-            buf ^= 1u;
+                for (int e = i * 4 / kOps; e < (i + 1) * 4 / kOps; e++)
+#pragma unroll
+                    for (int t = 0; t < RT; t++)
+                        sum[t] += weigh2<NP>(x[t][e / 2][e % 2 * 2], x[t][e / 2][e % 2 * 2 + 1], f[t], c[t], 2 * e, p[t]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int i = 0; i < kOps; i++) {
+                const h8 w = ops[i % kAhead];
+                if (i + kAhead < kOps) ops[i % kAhead] = vf[(i + kAhead) * 64];
+#pragma unroll
+                for (int t = 0; t < RT; t++)
+#pragma unroll
+                    for (int k = 0; k < NP; k++) st[t].o[i] = mfma(w, p[t][k], st[t].o[i]);
+                if (i % 2) put(s2, i / 2);                // block j + 2, where j - 1 was
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int t = 0; t < RT; t++) st[t].l = __builtin_fmaf(sum[t], inv, st[t].l);
+            fetch(j + 3);
             __syncthreads();
+        };
+        if (n) {
+            __syncthreads();                              // the part before is done with the ring
+#pragma unroll
+            for (int i = 0; i < 2 * NU; i++) put(0, i);
+            fetch(1);
+#pragma unroll
+            for (int i = 0; i < 2 * NU; i++) put(1, i);
+            fetch(2);
+            ksn = ks[0];
+            vsn = vs[0];
+            __syncthreads();
+            v4f x[RT][2], y[RT][2];
+            scores(0, x);
+            uint32_t slot = 0;
+            for (uint32_t j = 0;; j += 2) {
+                block(j, slot, x, y);
+                slot = slot == 2 ? 0u : slot + 1;
+                if (j + 1 >= n) break;
+                block(j + 1, slot, y, x);
+                slot = slot == 2 ? 0u : slot + 1;
+                if (j + 2 >= n) break;
+            }
         }
         const bool whole = c0 == 0 && nc == it.t.chunks;
         const uint64_t slot = (uint64_t)wg * 2 + (c0 ? 0u : 1u);
@@ -898,12 +938,12 @@ uint32_t tile_rows(Kind k)
     return k == kFew ? kFewM : k == kMany64 ? 64u : 128u;
 }
 
-template <int DP, int NP, int RT, int BT> int launch_many(Problem &a, uint32_t wgs, hipStream_t st)
+template <int DP, int NP, int RT> int launch_many(Problem &a, uint32_t wgs, hipStream_t st)
 {
-    const size_t lds = 2u * BT * 2u * DP * 4u * 16u;
-    hipLaunchKernelGGL((many_k<DP, NP, RT, BT>), dim3(wgs), dim3(256), lds, st, a);
+    const size_t lds = 3u * 2u * DP * 4u * 16u;
+    hipLaunchKernelGGL((many_k<DP, NP, RT>), dim3(wgs), dim3(256), lds, st, a);
     if (hipPeekAtLastError() != hipSuccess) return -1;
-    if (a.v.n_blocks > kChunk)
+    if (a.v.n_blocks > a.chunk)
         hipLaunchKernelGGL((merge_k<64 * RT, DP, false>), dim3(wgs - 1, 4), dim3(256), 0, st, a);
     return hipPeekAtLastError() == hipSuccess ? 0 : -1;
 }
@@ -916,17 +956,16 @@ template <int DP> int launch_dp(Problem &a, Kind kind, int n_cu, hipStream_t st)
         else hipLaunchKernelGGL((few_k<DP, 2>), dim3(wgs), dim3(256), 0, st, a);
         if (hipPeekAtLastError() != hipSuccess) return -1;
         // no item of a cache of one chunk is ever cut
-        if (a.v.n_blocks > kChunk) {
+        if (a.v.n_blocks > a.chunk) {
             const uint32_t rows = a.b.lens && !a.b.starts ? std::min(kFewM, a.n_rep) : kFewM;
             hipLaunchKernelGGL((merge_k<kFewM, DP, true>), dim3(wgs - 1, rows), dim3(256), 0, st, a);
         }
         return hipPeekAtLastError() == hipSuccess ? 0 : -1;
     }
-    constexpr int BT = DP <= 128 ? 2 : 1;
     if (kind == kMany64)
-        return a.q.f16 ? launch_many<DP, 1, 1, BT>(a, wgs, st) : launch_many<DP, 2, 1, BT>(a, wgs, st);
+        return a.q.f16 ? launch_many<DP, 1, 1>(a, wgs, st) : launch_many<DP, 2, 1>(a, wgs, st);
     if constexpr (DP <= 128)
-        return a.q.f16 ? launch_many<DP, 1, 2, BT>(a, wgs, st) : launch_many<DP, 2, 2, BT>(a, wgs, st);
+        return a.q.f16 ? launch_many<DP, 1, 2>(a, wgs, st) : launch_many<DP, 2, 2>(a, wgs, st);
     return -1;
 }
 
@@ -954,6 +993,13 @@ int launch_attention(const View &v, const Batch &b, uint32_t n_heads, const Rows
     a.sign = std::signbit(scale) ? -1.f : 1.f;
     a.scale2 = fabsf(scale) * 1.44269504f;
     const Kind kind = kind_of(v, b.n_rows, b.starts || !b.lens, a.n_rep);
+    while ((1ull << a.rep_shift) < a.n_rep) a.rep_shift++;
+    a.rep_mul = (uint32_t)((((1ull << a.rep_shift) - a.n_rep) << 32) / a.n_rep + 1);
+    // a block for each wave of few_k, two of many_k; more where the chunks
+    // would not be counted in 31 bits (all tiles seeing the whole cache)
+    a.chunk = kind == kFew ? 4u : 2u;
+    const uint64_t tiles = ((uint64_t)b.n_rows * a.n_rep + tile_rows(kind) - 1) / tile_rows(kind) + v.n_seqs;
+    while (tiles * v.n_heads * (v.n_blocks / a.chunk + 1) >> 31) a.chunk *= 2;
     a.w = work_at(work, workgroups(n_cu), tile_rows(kind));
     switch (v.dp) {
     case 64: return launch_dp<64>(a, kind, n_cu, st);
