@@ -11,97 +11,313 @@
 namespace qgl {
 namespace {
 
+// A row's numbers: m = max x, z = sum e, s = sum d e with d = (x - m) log2(e) and
+// e = 2^d, so that log p_t = x_t - m - ln z and the entropy is ln z - ln(2) s / z.
+//
+// A row is read once, in parts of one workgroup each (several where there are
+// few rows; joined by final_k), 256 E elements at a time in registers: the maximum
+// of a thread's own elements, then their sums under it, then the threads' sums
+// are joined.  For the alternatives every element is a key (value, then the
+// smaller id first), all keys distinct.  The k-th largest of the threads' largest
+// keys is a floor: no more than k threads hold keys at or above it, so at most k E
+// candidates leave the registers, usually little more than k; they are ranked by
+// counting the larger ones.
+//
+// Bound by the read of the logits where there are many rows, by two dependent
+// launches where there are few.
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kMaxParts = 64, kMaxK = QG_LOGPROBS_MAX_TOP;
+constexpr float kLowest = -3.402823466e38f, kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+
 struct Args {
     const void *x;
     uint64_t ld;
-    uint32_t f16, n_cols, n_given, k;
+    uint32_t n_cols, n_given, k;
+    uint32_t parts, len;             // elements of a part
     const uint32_t *tokens;
     float *logprobs, *entropy;
     uint32_t *top_ids;
     float *top_logprobs;
+    float *sums;                     // [row][part][4]: m, z, s
+    uint64_t *keys;                  // [row][part][k]
 };
 
-__device__ __forceinline__ float at(const Args &a, uint64_t row, uint32_t i)
+struct Sums {
+    float m, z, s;
+};
+
+// The sums of two sets of logits.  m is at least kLowest, so that a set of
+// nothing (or of -inf) adds nothing.
+__device__ __forceinline__ Sums join(Sums a, Sums b)
 {
-    return a.f16 ? (float)((const _Float16 *)a.x)[row * a.ld + i] : ((const float *)a.x)[row * a.ld + i];
+    const float m = fmaxf(a.m, b.m);
+    const float da = fmaxf(a.m - m, -1e30f) * kLog2e, db = fmaxf(b.m - m, -1e30f) * kLog2e;
+    // inf - inf is NaN and stays one
+    const float ea = __builtin_amdgcn_exp2f((a.m - m) * kLog2e), eb = __builtin_amdgcn_exp2f((b.m - m) * kLog2e);
+    return Sums{m, a.z * ea + b.z * eb, ea * (a.s + da * a.z) + eb * (b.s + db * b.z)};
 }
 
-// x before y among the alternatives: larger, or equal with a smaller id
-__device__ __forceinline__ bool before(float x, uint32_t i, float y, uint32_t j)
+// Over the workgroup, to all threads.
+__device__ Sums join_all(Sums a, Sums *red)
 {
-    return j == QG_TOKEN_NONE || x > y || (x == y && i < j);
-}
-
-template <class F> __device__ __forceinline__ float block_fold(float v, float *red, F f)
-{
-    for (int o = 32; o > 0; o >>= 1) v = f(v, __shfl_xor(v, o, 64));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        a = join(a, Sums{__shfl_xor(a.m, o, 64), __shfl_xor(a.z, o, 64), __shfl_xor(a.s, o, 64)});
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63u) == 0) red[threadIdx.x >> 6] = a;
     __syncthreads();
-    v = red[0];
-    for (uint32_t i = 1; i < blockDim.x >> 6; i++) v = f(v, red[i]);
-    return v;
+    a = red[0];
+#pragma unroll
+    for (uint32_t i = 1; i < kThreads / 64; i++) a = join(a, red[i]);
+    return a;
 }
 
-// One workgroup per row.
-__global__ void __launch_bounds__(256) row_k(Args a)
+// Larger keys first: larger values, then smaller ids.  0: no key (NaN).
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t id)
 {
-    __shared__ float red[4], bx[4];
-    __shared__ uint32_t bi[4];
+    const uint32_t b = __float_as_uint(x + 0.f);              // -0 as 0
+    const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
+    return x == x ? (uint64_t)o << 32 | (uint32_t)~id : 0ull;
+}
+__device__ __forceinline__ float value_of(uint64_t key)
+{
+    const uint32_t o = (uint32_t)(key >> 32);
+    return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+}
+
+// LDS of the selection: candidates, the threads' largest keys, the best so far,
+// floor_of's answer, the number of candidates.
+template <uint32_t CAP> struct Pick {
+    uint64_t cand[CAP], top[kThreads], best[kMaxK], floor;
+    uint32_t n;
+};
+
+// The k-th largest of the threads' keys (0: fewer than k have one).
+template <uint32_t CAP> __device__ uint64_t floor_of(Pick<CAP> &p, uint64_t key, uint32_t k)
+{
+    __syncthreads();
+    p.top[threadIdx.x] = key;
+    if (threadIdx.x == 0) p.floor = 0;
+    __syncthreads();
+    uint32_t larger = 0;
+    for (uint32_t i = 0; i < kThreads; i += 2) {
+        const ulonglong2 t = *(const ulonglong2 *)&p.top[i];
+        larger += (t.x > key ? 1u : 0u) + (t.y > key ? 1u : 0u);
+    }
+    if (key && larger == k - 1) p.floor = key;               // one thread, or none
+    __syncthreads();
+    return p.floor;
+}
+
+// The k largest of p.cand[0 .. p.n), in order, into p.best (0 behind them).
+template <uint32_t CAP> __device__ void rank(Pick<CAP> &p, uint32_t k)
+{
+    constexpr uint32_t R = (CAP + kThreads - 1) / kThreads;
+    __syncthreads();
+    while (p.n > kThreads) {                                  // at most k R are left each time
+        uint64_t own[R], top = 0;
+        const uint32_t n = p.n;
+#pragma unroll
+        for (uint32_t i = 0; i < R; i++) {
+            const uint32_t at = threadIdx.x + i * kThreads;
+            own[i] = at < n ? p.cand[at] : 0ull;
+            top = own[i] > top ? own[i] : top;
+        }
+        const uint64_t f = floor_of(p, top, k);
+        if (threadIdx.x == 0) p.n = 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < R; i++)
+            if (own[i] && own[i] >= f) p.cand[atomicAdd(&p.n, 1u)] = own[i];
+        __syncthreads();
+    }
+    const uint32_t n = p.n;
+    const uint64_t own = threadIdx.x < n ? p.cand[threadIdx.x] : 0ull;
+    uint32_t larger = 0;
+    for (uint32_t i = 0; i < n; i++) larger += p.cand[i] > own ? 1u : 0u;
+    __syncthreads();
+    if (threadIdx.x < k) p.best[threadIdx.x] = 0;
+    __syncthreads();
+    if (own && larger < k) p.best[larger] = own;
+    __syncthreads();
+}
+
+// What a row answers with, from its sums and the keys in `best`.
+__device__ void answer(const Args &a, uint64_t row, const void *x, bool f16, Sums t, const uint64_t *best)
+{
+    // no token of positive probability: no distribution
+    const float lz = t.z > 0.f ? logf(t.z) : __uint_as_float(0x7FC00000u);
+    for (uint32_t i = threadIdx.x; i < a.n_given; i += kThreads) {
+        const uint32_t id = a.tokens[row * a.n_given + i];
+        float y = id == QG_TOKEN_NONE ? 0.f : __uint_as_float(0x7FC00000u);
+        if (id < a.n_cols) y = (f16 ? (float)((const _Float16 *)x)[id] : ((const float *)x)[id]) - t.m - lz;
+        a.logprobs[row * a.n_given + i] = y;
+    }
+    if (a.entropy && threadIdx.x == 0) a.entropy[row] = lz - kLn2 * (t.s / t.z);
+    for (uint32_t i = threadIdx.x; i < a.k; i += kThreads) {
+        const uint64_t key = best[i];
+        a.top_ids[row * a.k + i] = key ? ~(uint32_t)key : QG_TOKEN_NONE;
+        a.top_logprobs[row * a.k + i] = key ? value_of(key) - t.m - lz : -INFINITY;
+    }
+}
+
+// Grid: (rows, parts).  TOP: with alternatives.
+template <int E, bool F16, bool TOP> __global__ void __launch_bounds__(kThreads) part_k(Args a)
+{
+    constexpr uint32_t VE = F16 ? 8 : 4, NV = E / VE, CAP = TOP ? kMaxK * E + kMaxK : 1;
+    __shared__ __attribute__((aligned(16))) Pick<CAP> pick;
+    __shared__ Sums red[kThreads / 64];
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
     const uint64_t row = blockIdx.x;
-    float m = -INFINITY;
-    for (uint32_t i = threadIdx.x; i < a.n_cols; i += 256) m = fmaxf(m, at(a, row, i));
-    m = block_fold(m, red, [](float x, float y) { return fmaxf(x, y); });
-    float z = 0.f, s = 0.f;
-    for (uint32_t i = threadIdx.x; i < a.n_cols; i += 256) {
-        const float d = at(a, row, i) - m, e = expf(d);
-        z += e;
-        if (!(e == 0.f)) s += d * e;
-    }
-    z = block_fold(z, red, [](float x, float y) { return x + y; });
-    s = block_fold(s, red, [](float x, float y) { return x + y; });
-    const float lz = logf(z);
-    for (uint32_t i = threadIdx.x; i < a.n_given; i += 256) {
-        const uint32_t t = a.tokens[row * a.n_given + i];
-        a.logprobs[row * a.n_given + i] = t == QG_TOKEN_NONE ? 0.f : t < a.n_cols ? at(a, row, t) - m - lz : NAN;
-    }
-    if (a.entropy && threadIdx.x == 0) a.entropy[row] = lz - s / z;
-    float px = INFINITY;
-    uint32_t pi = QG_TOKEN_NONE;
-    for (uint32_t r = 0; r < a.k; r++) {
-        float x = -INFINITY;
-        uint32_t id = QG_TOKEN_NONE;
-        for (uint32_t i = threadIdx.x; i < a.n_cols; i += 256) {
-            const float y = at(a, row, i);
-            // behind the last one taken (r > 0), a number, and before the best so far
-            if (y == y && (r == 0 || before(px, pi, y, i)) && (r == 0 || i != pi) && before(y, i, x, id)) { x = y; id = i; }
-        }
-        for (int o = 32; o > 0; o >>= 1) {
-            const float ox = __shfl_xor(x, o, 64);
-            const uint32_t oi = (uint32_t)__shfl_xor((int)id, o, 64);
-            if (oi != QG_TOKEN_NONE && before(ox, oi, x, id)) { x = ox; id = oi; }
-        }
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) { bx[threadIdx.x >> 6] = x; bi[threadIdx.x >> 6] = id; }
-        __syncthreads();
-        x = bx[0];
-        id = bi[0];
-        for (int i = 1; i < 4; i++)
-            if (bi[i] != QG_TOKEN_NONE && before(bx[i], bi[i], x, id)) { x = bx[i]; id = bi[i]; }
-        if (threadIdx.x == 0) {
-            a.top_ids[row * a.k + r] = id;
-            a.top_logprobs[row * a.k + r] = id == QG_TOKEN_NONE ? -INFINITY : x - m - lz;
-        }
-        px = x;
-        pi = id;
-        if (id == QG_TOKEN_NONE) {
-            for (uint32_t j = r + 1 + threadIdx.x; j < a.k; j += 256) {
-                a.top_ids[row * a.k + j] = QG_TOKEN_NONE;
-                a.top_logprobs[row * a.k + j] = -INFINITY;
+    const uint32_t es = F16 ? 2 : 4, lo = blockIdx.y * a.len, hi = min(lo + a.len, a.n_cols);
+    const char *x = (const char *)a.x + row * a.ld * es;
+    // the first element of a 16-byte word at or before lo
+    const int64_t begin = (int64_t)lo - (int64_t)(((uintptr_t)x / es + lo) % VE);
+    Sums all{kLowest, 0.f, 0.f};
+    uint64_t least = 0;                                        // the k-th best so far
+    if (TOP && threadIdx.x < kMaxK) pick.best[threadIdx.x] = 0;
+    for (int64_t c = begin; c < (int64_t)hi; c += (int64_t)kThreads * E) {
+        float v[NV][VE];
+#pragma unroll
+        for (uint32_t i = 0; i < NV; i++) {
+            const int64_t at = c + (int64_t)(i * kThreads + threadIdx.x) * VE;
+            if (at >= (int64_t)lo && at + VE <= (int64_t)hi) {
+                if (F16) {
+                    const h8 w = *(const h8 *)(x + at * 2);
+#pragma unroll
+                    for (uint32_t j = 0; j < VE; j++) v[i][j] = (float)w[j];
+                } else {
+                    const float4 w = *(const float4 *)(x + at * 4);
+                    v[i][0] = w.x; v[i][1] = w.y; v[i][2] = w.z; v[i][3] = w.w;
+                }
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < VE; j++) {
+                    const int64_t k = at + j;
+                    v[i][j] = k < (int64_t)lo || k >= (int64_t)hi ? -INFINITY
+                              : F16 ? (float)((const _Float16 *)x)[k] : ((const float *)x)[k];
+                }
             }
-            break;
+        }
+        Sums t{kLowest, 0.f, 0.f};
+#pragma unroll
+        for (uint32_t i = 0; i < NV; i++)
+#pragma unroll
+            for (uint32_t j = 0; j < VE; j++) t.m = fmaxf(t.m, v[i][j]);
+#pragma unroll
+        for (uint32_t i = 0; i < NV; i++)
+#pragma unroll
+            for (uint32_t j = 0; j < VE; j++) {
+                const float d = (v[i][j] - t.m) * kLog2e, e = __builtin_amdgcn_exp2f(d);
+                t.z += e;
+                t.s = __builtin_fmaf(fmaxf(d, -1000.f), e, t.s);
+            }
+        all = join(all, t);
+        if (TOP) {
+            const int64_t own0 = c + (int64_t)threadIdx.x * VE;
+            auto inside = [&](uint32_t i, uint32_t j, uint32_t *id) {
+                const int64_t k = own0 + (int64_t)i * kThreads * VE + j;
+                *id = (uint32_t)k;
+                return k >= (int64_t)lo && k < (int64_t)hi;
+            };
+            // the thread's largest key: the first of its largest values (t.m is
+            // kLowest at least: such rows look at every element)
+            uint64_t top = 0;
+            if (t.m > kLowest) {
+#pragma unroll
+                for (int i = NV - 1; i >= 0; i--)
+#pragma unroll
+                    for (int j = VE - 1; j >= 0; j--) {
+                        uint32_t id;
+                        (void)inside(i, j, &id);
+                        if (v[i][j] == t.m) top = key_of(t.m, id);
+                    }
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < NV; i++)
+#pragma unroll
+                    for (uint32_t j = 0; j < VE; j++) {
+                        uint32_t id;
+                        const uint64_t key = inside(i, j, &id) ? key_of(v[i][j], id) : 0ull;
+                        top = key > top ? key : top;
+                    }
+            }
+            if (__syncthreads_or(top > least)) {
+                const uint64_t f = floor_of(pick, top, a.k);
+                const uint64_t from = f > least ? f : least + 1;
+                if (threadIdx.x == 0) pick.n = 0;
+                __syncthreads();
+                if (threadIdx.x < a.k && pick.best[threadIdx.x])
+                    pick.cand[atomicAdd(&pick.n, 1u)] = pick.best[threadIdx.x];
+                if (top >= from)
+#pragma unroll
+                    for (uint32_t i = 0; i < NV; i++)
+#pragma unroll
+                        for (uint32_t j = 0; j < VE; j++) {
+                            uint32_t id;
+                            const uint64_t key = inside(i, j, &id) ? key_of(v[i][j], id) : 0ull;
+                            if (key >= from) pick.cand[atomicAdd(&pick.n, 1u)] = key;
+                        }
+                rank(pick, a.k);
+                least = pick.best[a.k - 1];
+            }
         }
     }
+    all = join_all(all, red);
+    if (a.parts == 1) {
+        answer(a, row, x, F16, all, TOP ? pick.best : nullptr);
+        return;
+    }
+    const uint64_t at = row * a.parts + blockIdx.y;
+    if (threadIdx.x == 0) *(float4 *)(a.sums + at * 4) = make_float4(all.m, all.z, all.s, 0.f);
+    if (TOP && threadIdx.x < a.k) a.keys[at * a.k + threadIdx.x] = pick.best[threadIdx.x];
+}
+
+// Joins the parts of a row.
+template <bool F16, bool TOP> __global__ void __launch_bounds__(kThreads) final_k(Args a)
+{
+    constexpr uint32_t CAP = TOP ? kMaxParts * kMaxK : 1;
+    __shared__ __attribute__((aligned(16))) Pick<CAP> pick;
+    __shared__ Sums red[kThreads / 64];
+    const uint64_t row = blockIdx.x;
+    Sums t{kLowest, 0.f, 0.f};
+    if (threadIdx.x < a.parts) {
+        const float4 w = *(const float4 *)(a.sums + (row * a.parts + threadIdx.x) * 4);
+        t = Sums{w.x, w.y, w.z};
+    }
+    if (TOP) {
+        if (threadIdx.x == 0) pick.n = 0;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < a.parts * a.k; i += kThreads) {
+            const uint64_t key = a.keys[row * a.parts * a.k + i];
+            if (key) pick.cand[atomicAdd(&pick.n, 1u)] = key;
+        }
+        rank(pick, a.k);
+    }
+    t = join_all(t, red);
+    answer(a, row, (const char *)a.x + row * a.ld * (F16 ? 2 : 4), F16, t, TOP ? pick.best : nullptr);
+}
+
+// Parts of a row: enough for about two workgroups per compute unit, of 2048
+// elements at least.
+uint32_t parts_of(size_t n_rows, size_t n_cols, int n_cu)
+{
+    const size_t want = 2u * (size_t)(n_cu > 0 ? n_cu : 256) / (n_rows ? n_rows : 1), most = (n_cols + 2047) / 2048;
+    size_t s = want < most ? want : most;
+    s = s < 1 ? 1 : s > kMaxParts ? kMaxParts : s;
+    return (uint32_t)s;
+}
+
+template <bool F16, bool TOP> void launch(const Args &a, uint32_t n_rows, hipStream_t st)
+{
+    const dim3 grid(n_rows, a.parts), block(kThreads);
+    // up to 7 elements more for the rows' alignment
+    const uint32_t per = (a.len + 7 + kThreads - 1) / kThreads;
+    if (per <= 8) hipLaunchKernelGGL((part_k<8, F16, TOP>), grid, block, 0, st, a);
+    else if (per <= 16) hipLaunchKernelGGL((part_k<16, F16, TOP>), grid, block, 0, st, a);
+    else if (per <= 32) hipLaunchKernelGGL((part_k<32, F16, TOP>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((part_k<64, F16, TOP>), grid, block, 0, st, a);
+    if (a.parts > 1) hipLaunchKernelGGL((final_k<F16, TOP>), dim3(n_rows), block, 0, st, a);
 }
 
 }  // namespace
@@ -114,7 +330,10 @@ int qg_logprobs_work(qg_ctx *ctx, size_t n_rows, size_t n_cols, size_t k, size_t
     if (!ctx || !bytes) return qg_fail(ctx, QG_ERR_INVALID_ARG, "ctx or bytes is NULL");
     if (n_rows > 0x7FFFFFFFu || n_cols < 1 || n_cols > 0x7FFFFFFFu || k > QG_LOGPROBS_MAX_TOP)
         return qg_fail(ctx, QG_ERR_SHAPE, "logits or alternatives");
-    *bytes = 0;
+    // what calls of fewer rows need too: parts * rows is largest just before the
+    // rows alone are enough workgroups
+    const size_t cus = (size_t)(ctx->n_cu > 0 ? ctx->n_cu : 256), cells = n_rows * qgl::kMaxParts;
+    *bytes = n_cols > 2048 ? (cells < 2 * cus ? cells : 2 * cus) * (16 + 8 * k) : 0;
     return QG_OK;
 }
 
@@ -146,7 +365,6 @@ int qg_logprobs_dev(qg_ctx *ctx, const void *d_logits, uint32_t type, size_t n_r
     qgl::Args a{};
     a.x = d_logits;
     a.ld = ld;
-    a.f16 = type == qg::T_F16;
     a.n_cols = (uint32_t)n_cols;
     a.n_given = (uint32_t)n_given;
     a.k = (uint32_t)k;
@@ -155,7 +373,13 @@ int qg_logprobs_dev(qg_ctx *ctx, const void *d_logits, uint32_t type, size_t n_r
     a.entropy = d_entropy;
     a.top_ids = d_top_ids;
     a.top_logprobs = d_top_logprobs;
-    hipLaunchKernelGGL(qgl::row_k, dim3((uint32_t)n_rows), dim3(256), 0, stream ? (hipStream_t)stream : ctx->stream, a);
+    a.parts = qgl::parts_of(n_rows, n_cols, ctx->n_cu);
+    a.len = (uint32_t)((n_cols + a.parts - 1) / a.parts);
+    a.sums = (float *)d_work;
+    a.keys = (uint64_t *)(a.sums + (size_t)n_rows * a.parts * 4);
+    const hipStream_t st = stream ? (hipStream_t)stream : ctx->stream;
+    if (type == qg::T_F16) k ? qgl::launch<true, true>(a, (uint32_t)n_rows, st) : qgl::launch<true, false>(a, (uint32_t)n_rows, st);
+    else k ? qgl::launch<false, true>(a, (uint32_t)n_rows, st) : qgl::launch<false, false>(a, (uint32_t)n_rows, st);
     e = hipGetLastError();
     return e == hipSuccess ? QG_OK : qg_fail(ctx, QG_ERR_HIP, "log probabilities", e);
 }

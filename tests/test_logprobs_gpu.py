@@ -67,8 +67,11 @@ def close(got, want, tol):
     assert not bad.any(), (np.abs(got[ok] - want[ok]).max(), tol[ok].min())
 
 
-def check(ctx, x, tokens=None, k=0, **kw):
+def check(ctx, x, tokens=None, k=0, first=None, **kw):
+    """Every row of a call, or its first ones."""
     lp, ent, ids, tl = call(ctx, x, tokens, k, **kw)
+    x, lp, ent, ids, tl = (y[:first] for y in (x, lp, ent, ids, tl))
+    tokens = None if tokens is None else tokens[:first]
     wlp, went = definition(x)
     n = x.shape[1]
     # f32 steps of x itself do not enter: they are the operator's input
@@ -86,7 +89,8 @@ def check(ctx, x, tokens=None, k=0, **kw):
         np.testing.assert_array_equal(ids[r], full)
         wt = np.full(k, -np.inf)
         wt[:len(want)] = wlp[r, want]
-        close(tl[r:r + 1], wt[None], near(wt[None]) if len(x) == 1 else near(np.tile(wt, (len(x), 1)))[r:r + 1])
+        big = np.abs(np.max(np.where(np.isfinite(x[r]), x[r], 0).astype(np.float64)))
+        close(tl[r], wt, 4 * U * np.abs(wt) + 4 * U * big + 2.0 ** -16)
 
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
@@ -116,6 +120,25 @@ def test_ties_and_orders(rinf, ctx, n, k):
     x = np.stack([rng.integers(0, 4, n), np.zeros(n), np.arange(n) / 512.0, -np.arange(n) / 512.0, -np.abs(np.arange(n) - n // 2) // 3,
                   np.where(np.arange(n) % 2, 0.0, -0.0)]).astype(np.float32)
     check(ctx, x, rng.integers(0, n, (len(x), 1)).astype(np.uint32), k)
+
+
+def test_long_parts(rinf, ctx):
+    """So many rows that one workgroup takes a row, in several pieces of 16384: the alternatives are
+    carried from piece to piece, also where every piece is better (rising) or none is (falling)."""
+    rng = np.random.default_rng(12)
+    rows, n = 600, 40003
+    for dtype in (np.float32, np.float16):
+        x = (rng.standard_normal((rows, n)) * 3).astype(dtype)
+        x[0], x[1] = np.arange(n) / 64.0, -np.arange(n) / 64.0
+        x[2], x[3] = 1.0, rng.integers(0, 3, n)
+        x[4, :30000], x[5, 16000:] = -np.inf, -np.inf
+        x[6], x[7] = -np.inf, np.nan
+        x[8, 39000:] += 20
+        x[9] = np.nan
+        x[9, [5, 17000, 40000]] = -np.inf, 2.0, 1.0
+        tokens = rng.integers(0, n, (rows, 1)).astype(np.uint32)
+        check(ctx, x, tokens, 64, first=16)
+        check(ctx, x, tokens, 3, first=16, ld=n + 1, off=3)
 
 
 def test_masked(rinf, ctx):
