@@ -125,6 +125,27 @@ int qg_model_set_attention_path(qg_model *m, int path);
  * only when it is also the lm_head).  Any output may be NULL. */
 int qg_model_resident_bytes(qg_model *m, size_t *weights, size_t *file_bytes, size_t *total);
 
+/* No counterpart in the reference: keep the KV caches in 8 bits (enable != 0;
+ * qg_kv8 of qgops.h, one per layer) instead of f32, in about a quarter of the
+ * memory: the decode step and both prefills then quantise their keys and values
+ * as they are written and attend over the codes (any head_dim up to 256, any
+ * length; QG_ERR_SHAPE beyond).  Tokens of one prefill chunk see the caches as
+ * they are when the chunk is written, so a block's scale may come from a later
+ * token of it: a prompt's logits and those of its tokens one by one differ by
+ * the order of what the quantisation changes.  The caches become empty, as by
+ * qg_model_reset, also when nothing changes.  On QG_ERR_OUT_OF_MEMORY the model
+ * keeps the caches it has. */
+int qg_model_use_kv8(qg_model *m, int enable);
+
+/* No counterpart in the reference: what the device logits of the last forward
+ * (before qg_model_sample_greedy, whose penalty changes them) say as
+ * probabilities, as qg_logprobs_dev (qgops.h) for one row: the log probability
+ * of each of n tokens into logprobs[n], the entropy into *entropy (may be
+ * NULL), the k <= 64 most likely tokens into top_ids[k] and top_logprobs[k].
+ * Host arrays; synchronous. */
+int qg_model_logprobs(qg_model *m, const uint32_t *tokens, size_t n, float *logprobs, float *entropy, size_t k,
+                      uint32_t *top_ids, float *top_logprobs);
+
 /* Greedy Sampler::sample on the device logits of the last forward:
  * repetition penalty over `recent` (the last `window` entries, applied in
  * order, sampler.rs:109-127) then argmax (math.rs:328-339).  Modifies the

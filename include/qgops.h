@@ -103,7 +103,8 @@ int qg_kv8_read_dev(qg_ctx *ctx, const qg_kv8 *kv, size_t seq, size_t n_seqs, si
  * cached values, this call's tokens' among them (qg_kv8_write_dev first):
  *   out = sum_j p_j v_j,  p = softmax over j of scale * q . k_j,
  * for the row at position p over the positions j <= p, and j > p - window
- * where window is not 0.  A row with no position to see (one below 0) gives
+ * where window is not 0.  Rows see the values as they are after the call's
+ * writes: a later token of the same block may have moved its scale.  A row with no position to see (one below 0) gives
  * zeros; a row at a position past max_len sees the positions there are.  q and
  * out have one type; f32 rows are computed to f32 precision (two f16 pieces of
  * q and of p), f16 rows with f16 p, sums in f32.  d_work: qg_kv8_attention_work

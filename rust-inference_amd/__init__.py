@@ -132,6 +132,8 @@ _SIGS = {
     "qg_model_use_batched_prefill": (ctypes.c_int, [_P, ctypes.c_int]),
     "qg_model_set_attention_path": (ctypes.c_int, [_P, ctypes.c_int]),
     "qg_model_resident_bytes": (ctypes.c_int, [_P, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)]),
+    "qg_model_use_kv8": (ctypes.c_int, [_P, ctypes.c_int]),
+    "qg_model_logprobs": (ctypes.c_int, [_P, _P, _SZ, _P, _P, _SZ, _P, _P]),
     "qg_model_sample_greedy": (ctypes.c_int, [_P, _P, _SZ, ctypes.c_float, _SZ, ctypes.POINTER(_U32)]),
     "qg_model_generate": (ctypes.c_int, [_P, _P, _SZ, _SZ, ctypes.c_float, _SZ, _P,
                                          ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]),
@@ -772,6 +774,22 @@ class DeviceModel:
         320 or 480 of them (head_dim 64, 128, 256); beyond, split), 1: always one workgroup per head, 2: always split over
         position ranges, 3: always two workgroups per head where allowed."""
         self.ctx.check(self.ctx.lib.qg_model_set_attention_path(self.h, int(path)), "qg_model_set_attention_path")
+
+    def use_kv8(self, enable: bool):
+        """KV caches in 8 bits (Kv8Cache's format) instead of f32; empties them (qg_model_use_kv8)."""
+        self.ctx.check(self.ctx.lib.qg_model_use_kv8(self.h, int(bool(enable))), "qg_model_use_kv8")
+
+    def logprobs(self, tokens=(), k: int = 0):
+        """(log probabilities of tokens, entropy, ids of the k most likely tokens,
+        their log probabilities) under the last forward's logits (qg_model_logprobs)."""
+        import numpy as np
+        t = np.ascontiguousarray(tokens, dtype=np.uint32)
+        lp, ent = np.zeros(len(t), np.float32), np.zeros(1, np.float32)
+        ids, top = np.zeros(k, np.uint32), np.zeros(k, np.float32)
+        self.ctx.check(self.ctx.lib.qg_model_logprobs(self.h, _ptr(t) if len(t) else None, len(t),
+                                                      _ptr(lp) if len(t) else None, _ptr(ent), k, _ptr(ids) if k else None,
+                                                      _ptr(top) if k else None), "qg_model_logprobs")
+        return lp, float(ent[0]), ids, top
 
     def forward(self, token: int, pos: int, logits=None):
         """logits: numpy float32[vocab] receiving the step's logits, or None."""

@@ -24,6 +24,8 @@
 //                    rescaled)
 //   qkv_post_k       the bias add, RoPE and KV append alone, and
 //   attention_k      attention in one workgroup per head (other head_dim)
+//   qkv_rope_k       the bias add and RoPE alone, before the 8-bit caches' write and
+//                    attention (qg_kv8.hip, qg_kv8_attention.hip; qg_model_use_kv8)
 //   SiLU * up        mlp.rs:31-43, silu as math.rs:137-146, in the epilogue
 //                    of the [gate; up] GEMV (gate and up rows paired), else
 //                    inside the down GEMV's prologue or a separate kernel
@@ -40,7 +42,9 @@
 
 #include "qg_common.h"
 #include "qg_internal.h"
+#include "qg_kv8.h"
 #include "qgmodel.h"
+#include "qgops.h"
 
 namespace qgm {
 
@@ -162,6 +166,35 @@ __global__ void __launch_bounds__(256) qkv_post_k(float *__restrict__ q, const f
         kr[i0 + 1] = x0 * s + x1 * c;
         vr[i0] = v[i0] + bv[i0];
         vr[i0 + 1] = v[i0 + 1] + bv[i0 + 1];
+    }
+}
+
+// The same without a cache to append to (8-bit caches): k and v in place, and
+// the number of positions with this one.
+__global__ void __launch_bounds__(256) qkv_rope_k(float *__restrict__ q, float *__restrict__ k, float *__restrict__ v,
+                                                  const float *__restrict__ bq, const float *__restrict__ bk,
+                                                  const float *__restrict__ bv, const float *__restrict__ cos_t,
+                                                  const float *__restrict__ sin_t, uint32_t q_dim, uint32_t kv_dim,
+                                                  uint32_t hd, const Step *__restrict__ st, uint32_t *__restrict__ len)
+{
+    const uint32_t t = blockIdx.x * blockDim.x + threadIdx.x, half = hd / 2;
+    const uint32_t pos = st->pos, i0 = 2 * t;
+    if (t == 0) *len = st->slot + 1;
+    if (i0 < q_dim) {
+        const uint32_t j = (i0 % hd) / 2;
+        const float c = cos_t[(size_t)pos * half + j], s = sin_t[(size_t)pos * half + j];
+        const float x0 = q[i0] + bq[i0], x1 = q[i0 + 1] + bq[i0 + 1];
+        q[i0] = x0 * c - x1 * s;
+        q[i0 + 1] = x0 * s + x1 * c;
+    }
+    if (i0 < kv_dim) {
+        const uint32_t j = (i0 % hd) / 2;
+        const float c = cos_t[(size_t)pos * half + j], s = sin_t[(size_t)pos * half + j];
+        const float x0 = k[i0] + bk[i0], x1 = k[i0 + 1] + bk[i0 + 1];
+        k[i0] = x0 * c - x1 * s;
+        k[i0 + 1] = x0 * s + x1 * c;
+        v[i0] += bv[i0];
+        v[i0 + 1] += bv[i0 + 1];
     }
 }
 
@@ -985,6 +1018,7 @@ __global__ void advance_k(Step *st, const uint32_t *hist)
 namespace {
 constexpr int kSlots = 7;                 // WQ .. DOWN
 constexpr uint32_t kRing = 256;           // pinned Step records for host-fed forwards
+constexpr size_t kGiven = 1024;           // tokens qg_model_logprobs takes at a time
 }
 
 struct qg_model {
@@ -1002,7 +1036,19 @@ struct qg_model {
     std::vector<bool> owned[kSlots];
     float *final_norm = nullptr;
     std::vector<float *> vec[6];          // per layer: attn_norm, ffn_norm, bq, bk, bv (slot 0 unused)
-    float *kc = nullptr, *vc = nullptr;   // [n_layers][max_seq_len][kv_dim]
+    float *kc = nullptr, *vc = nullptr;   // [n_layers][max_seq_len][kv_dim]; NULL with 8-bit caches
+    // 8-bit caches, one per layer (qg_model_use_kv8), the positions they hold, a
+    // prefill chunk's keys and values before they are quantised, the
+    // attention's workspace
+    std::vector<qg_kv8 *> kv8;
+    uint32_t *kv8_len = nullptr;
+    float *kv8_k = nullptr, *kv8_v = nullptr;
+    uint8_t *kv8_work = nullptr;
+    // qg_model_logprobs: tokens, log probabilities, entropy, alternatives, workspace
+    uint32_t *lp_tok = nullptr, *lp_ids = nullptr;
+    float *lp_out = nullptr, *lp_ent = nullptr, *lp_top = nullptr;
+    uint8_t *lp_work = nullptr;
+    size_t lp_work_bytes = 0;
     size_t seq = 0;
     float *cos_t = nullptr, *sin_t = nullptr;
     float *h0 = nullptr, *h1 = nullptr, *xn = nullptr, *q = nullptr, *k = nullptr, *v = nullptr;
@@ -1109,6 +1155,16 @@ void undo_allocs(qg_model *m, size_t held, size_t bytes)
     (void)hipStreamSynchronize(m->ctx->stream);
     for (; m->allocs.size() > held; m->allocs.pop_back()) (void)hipFree(m->allocs.back());
     m->alloc_bytes = bytes;
+}
+
+// Frees what dalloc handed out as *p (the caller has waited for its users).
+template <class T> void dfree(qg_model *m, T **p, size_t n)
+{
+    if (!*p) return;
+    m->allocs.erase(std::find(m->allocs.begin(), m->allocs.end(), (void *)*p));
+    m->alloc_bytes -= (n ? n : 1) * sizeof(T);
+    (void)hipFree(*p);
+    *p = nullptr;
 }
 
 // hipMemcpy in the order of the context's stream, and waited for.  The legacy
@@ -1239,6 +1295,7 @@ void free_model(qg_model *m)
     const bool alias = lm_alias(m);
     qg_mat_release(m->ctx, m->tok, m->tok_owned);
     if (!alias) qg_mat_release(m->ctx, m->lm, m->lm_owned);
+    for (qg_kv8 *kv : m->kv8) qg_kv8_drop(kv);
     for (void *p : m->allocs) (void)hipFree(p);
     if (m->h_recent) (void)hipHostFree(m->h_recent);
     if (m->h_token) (void)hipHostFree(m->h_token);
@@ -1310,6 +1367,30 @@ int gemv_norm(qg_model *m, const qg_mat *A, const float *xa, const float *xb, co
     return qg_norm_matvec(m->ctx, A, xa, xb, nw, m->cfg.norm_eps, sum_out, y, m->xn, m->ctx->stream);
 }
 
+// n rows of `heads` heads of the model's f32 activations
+qg8::Rows kv8_rows(const qg_model *m, const float *p, size_t ld)
+{
+    qg8::Rows r{};
+    r.p = const_cast<float *>(p);
+    r.ld_row = ld;
+    r.ld_head = m->hd;
+    r.vec = (uintptr_t)p % 16 == 0 && ld % 4 == 0 && m->hd % 16 == 0;
+    return r;
+}
+
+// Caches the rows' k and v in layer l and attends: the positions end at
+// b.len0 or, for the decode step's one row, at *kv8_len.
+int kv8_attention(qg_model *m, uint32_t l, const qg8::Batch &b, const float *q, size_t ldq, const float *k, size_t ldk,
+                  const float *v, size_t ldv, float *out)
+{
+    const qg8::View &c = m->kv8[l]->v;
+    if (qg8::launch_write(c, b, kv8_rows(m, k, ldk), kv8_rows(m, v, ldv), m->ctx->stream) ||
+        qg8::launch_attention(c, b, m->cfg.n_heads, kv8_rows(m, q, ldq), 1.0f / sqrtf((float)m->hd), 0,
+                              kv8_rows(m, out, m->q_dim), m->kv8_work, m->ctx->n_cu, m->ctx->stream))
+        return mfail(m, QG_ERR_HIP, "attention over the 8-bit cache", hipGetLastError());
+    return QG_OK;
+}
+
 int launched(qg_model *m, const char *what)
 {
     hipError_t e = hipGetLastError();
@@ -1373,7 +1454,14 @@ int enqueue_forward(qg_model *m)
             return rc;
         }
         float *kc = m->kc + l * kv_layer, *vc = m->vc + l * kv_layer;
-        if (m->att_grp) {
+        if (!m->kv8.empty()) {
+            hipLaunchKernelGGL(qgm::qkv_rope_k, dim3((pairs + 255) / 256), dim3(256), 0, st, m->q, m->k, m->v,
+                               m->vec[QG_V_BQ][l], m->vec[QG_V_BK][l], m->vec[QG_V_BV][l], m->cos_t, m->sin_t, m->q_dim,
+                               m->kv_dim, m->hd, m->d_step, m->kv8_len);
+            if ((rc = kv8_attention(m, l, qg8::Batch{nullptr, m->kv8_len, 1, 0}, m->q, m->q_dim, m->k, m->kv_dim, m->v,
+                                    m->kv_dim, m->ao)))
+                return rc;
+        } else if (m->att_grp) {
             qgm::AttnArgs aa{};
             aa.q = m->q; aa.k = m->k; aa.v = m->v;
             aa.bq = m->vec[QG_V_BQ][l]; aa.bk = m->vec[QG_V_BK][l]; aa.bv = m->vec[QG_V_BV][l];
@@ -1542,6 +1630,10 @@ bool two_range_ok(const qg_model *m)
 // workgroup per head).
 void pick_attention(qg_model *m, uint32_t slot)
 {
+    if (!m->kv8.empty()) {                       // one sequence of launches for every length
+        m->att_mode = 0;
+        return;
+    }
     const int whole = m->att_path != 1 && two_range_ok(m) ? 2 : 1;
     const uint32_t most = whole == 2 ? qgm::kShortSeq : qgm::short_seq1(m->hd);
     const bool shrt = m->att_path == 1 || m->att_path == 3 || (m->att_path == 0 && slot + 1 <= most);
@@ -1729,14 +1821,18 @@ int pf_chunk(qg_model *m, const uint32_t *d_tok, uint32_t ntok, uint32_t s0, boo
         } else if ((rc = pf_gemm(m, qkv, 3, E, ntok, ldq, s_qk))) {
             return rc;
         }
-        float *kc = m->kc + l * kv_layer, *vc = m->vc + l * kv_layer;
+        const bool kv8 = !m->kv8.empty();          // keys and values in a buffer first
+        float *kc = kv8 ? m->kv8_k : m->kc + l * kv_layer, *vc = kv8 ? m->kv8_v : m->vc + l * kv_layer;
         if (qg::launch_pf_qkv_post(m->pf_qkv, ldq, s_qk, T * ldq, m->pf_qkv + m->q_dim + m->kv_dim, ldq, s_v, T * ldq,
                                    m->pf_ss, E, c.norm_eps,
                                    m->vec[QG_V_BQ][l], m->vec[QG_V_BK][l], m->vec[QG_V_BV][l], kc, vc, m->cos_t,
-                                   m->sin_t, m->q_dim, m->kv_dim, m->hd, s0, s0, ntok, sti) ||
-            qg::launch_pf_attention(m->pf_qkv, ldq, kc, vc, m->pf_ao, c.n_heads, m->hd, m->kv_dim, m->n_rep, scale, s0,
-                                    ntok, sti))
+                                   m->sin_t, m->q_dim, m->kv_dim, m->hd, s0, kv8 ? 0 : s0, ntok, sti) ||
+            (!kv8 && qg::launch_pf_attention(m->pf_qkv, ldq, kc, vc, m->pf_ao, c.n_heads, m->hd, m->kv_dim, m->n_rep,
+                                             scale, s0, ntok, sti)))
             return mfail(m, QG_ERR_HIP, "prefill attention", hipGetLastError());
+        if (kv8 && (rc = kv8_attention(m, l, qg8::Batch{nullptr, nullptr, ntok, s0 + ntok}, m->pf_qkv, ldq, kc, m->kv_dim,
+                                       vc, m->kv_dim, m->pf_ao)))
+            return rc;
         const qg::PfMat wo = pf_mat(m->w[QG_M_WO - 2][l], m->pf_ao2);
         if ((rc = pf_planes(m, m->pf_ao, 1, nullptr, 0, nullptr, nullptr, m->q_dim, m->q_dim, 0, false, ntok)) ||
             (rc = pf_gemm(m, &wo, 1, m->q_dim, ntok, E, m->pf_s_o)))
@@ -1899,13 +1995,17 @@ int wide_chunk(qg_model *m, const uint32_t *d_tok, uint32_t ntok, uint32_t s0, b
         if ((rc = wide_gemm(m, qkv, v_apart ? 2 : 3, E, ntok, ldq, s_qk, T * ldq)) ||
             (v_apart && (rc = wide_gemm(m, qkv + 2, 1, E, ntok, ldv, s_v, T * ldv))))
             return rc;
-        float *kc = m->kc + l * kv_layer, *vc = m->vc + l * kv_layer;
+        const bool kv8 = !m->kv8.empty();
+        float *kc = kv8 ? m->kv8_k : m->kc + l * kv_layer, *vc = kv8 ? m->kv8_v : m->vc + l * kv_layer;
         if (qg::launch_pf_qkv_post(m->wd_qkv, ldq, s_qk, T * ldq, v, ldv, s_v, T * ldv, nullptr, E, c.norm_eps,
                                    m->vec[QG_V_BQ][l], m->vec[QG_V_BK][l], m->vec[QG_V_BV][l], kc, vc, m->cos_t, m->sin_t, m->q_dim,
-                                   m->kv_dim, m->hd, s0, s0, ntok, sti) ||
-            qg::launch_wide_attention(m->wd_qkv, ldq, kc, vc, m->wd_ao, c.n_heads, m->hd, m->kv_dim, m->n_rep, scale,
-                                      s0, ntok, sti))
+                                   m->kv_dim, m->hd, s0, kv8 ? 0 : s0, ntok, sti) ||
+            (!kv8 && qg::launch_wide_attention(m->wd_qkv, ldq, kc, vc, m->wd_ao, c.n_heads, m->hd, m->kv_dim, m->n_rep,
+                                               scale, s0, ntok, sti)))
             return mfail(m, QG_ERR_HIP, "prefill attention", hipGetLastError());
+        if (kv8 && (rc = kv8_attention(m, l, qg8::Batch{nullptr, nullptr, ntok, s0 + ntok}, m->wd_qkv, ldq, kc, m->kv_dim,
+                                       vc, m->kv_dim, m->wd_ao)))
+            return rc;
         const qg::PfMat wo = pf_mat(m->w[QG_M_WO - 2][l], m->wd_ao2);
         if ((rc = wide_planes(m, m->wd_ao, 1, nullptr, 0, 0, nullptr, nullptr, m->q_dim, m->q_dim, 0, ntok)) ||
             (rc = wide_gemm(m, &wo, 1, m->q_dim, ntok, E, sp.o, T * E)) ||
@@ -2237,7 +2337,112 @@ int qg_model_resident_bytes(qg_model *m, size_t *weights, size_t *file_bytes, si
     for (const qg_mat *p : m->f_gu) add(p, false);
     if (weights) *weights = w;
     if (file_bytes) *file_bytes = f;
-    if (total) *total = w + m->alloc_bytes;
+    size_t kv8 = 0;
+    for (const qg_kv8 *kv : m->kv8) kv8 += kv->bytes;
+    if (total) *total = w + m->alloc_bytes + kv8;
+    return QG_OK;
+}
+
+int qg_model_use_kv8(qg_model *m, int enable)
+{
+    if (!m) return QG_ERR_INVALID_ARG;
+    if ((enable != 0) == !m->kv8.empty()) {
+        m->seq = 0;
+        return QG_OK;
+    }
+    const qg_model_config &c = m->cfg;
+    if (enable && m->hd > 256) return mfail(m, QG_ERR_SHAPE, "8-bit caches hold heads of at most 256 elements");
+    QGM_HIP(m, hipSetDevice(m->ctx->device));
+    QGM_HIP(m, hipStreamSynchronize(m->ctx->stream));
+    const size_t kvn = (size_t)c.n_layers * c.max_seq_len * m->kv_dim;
+    const size_t rows = std::min<size_t>(c.max_seq_len, qg::kWideMax);
+    const size_t held = m->allocs.size(), bytes = m->alloc_bytes;
+    int rc = QG_OK;
+    if (!enable) {
+        if ((rc = dalloc(m, &m->kc, kvn)) || (rc = dalloc(m, &m->vc, kvn))) {
+            undo_allocs(m, held, bytes);
+            m->kc = m->vc = nullptr;
+            return rc;
+        }
+        for (qg_kv8 *kv : m->kv8) qg_kv8_drop(kv);
+        const size_t work = qg8::attention_work(m->kv8[0]->v, rows, c.n_heads, m->ctx->n_cu);
+        m->kv8.clear();
+        dfree(m, &m->kv8_len, 1);
+        dfree(m, &m->kv8_k, rows * m->kv_dim);
+        dfree(m, &m->kv8_v, rows * m->kv_dim);
+        dfree(m, &m->kv8_work, work);
+    } else {
+        // all of it, or the f32 caches stay
+        std::vector<qg_kv8 *> kv;
+        try {
+            kv.reserve(c.n_layers);
+            m->allocs.reserve(held + 4);
+        } catch (...) {
+            return mfail(m, QG_ERR_OUT_OF_MEMORY, "host allocation");
+        }
+        for (uint32_t l = 0; l < c.n_layers && !rc; l++) {
+            qg_kv8 *one = nullptr;
+            if (!(rc = qg_kv8_make(m->ctx, 1, c.n_kv_heads, m->hd, c.max_seq_len, &one))) kv.push_back(one);
+        }
+        if (!rc) rc = dalloc(m, &m->kv8_len, 1);
+        if (!rc) rc = dalloc(m, &m->kv8_k, rows * m->kv_dim);
+        if (!rc) rc = dalloc(m, &m->kv8_v, rows * m->kv_dim);
+        if (!rc) rc = dalloc(m, &m->kv8_work, qg8::attention_work(kv[0]->v, rows, c.n_heads, m->ctx->n_cu));
+        if (rc) {
+            undo_allocs(m, held, bytes);
+            m->kv8_len = nullptr;
+            m->kv8_k = m->kv8_v = nullptr;
+            m->kv8_work = nullptr;
+            for (qg_kv8 *one : kv) qg_kv8_drop(one);
+            return rc;
+        }
+        dfree(m, &m->kc, kvn);
+        dfree(m, &m->vc, kvn);
+        m->kv8.swap(kv);
+    }
+    drop_graphs(m);                              // they hold the other caches' launches
+    m->seq = 0;
+    return QG_OK;
+}
+
+int qg_model_logprobs(qg_model *m, const uint32_t *tokens, size_t n, float *logprobs, float *entropy, size_t k,
+                      uint32_t *top_ids, float *top_logprobs)
+{
+    if (!m || (n && (!tokens || !logprobs)) || (k && (!top_ids || !top_logprobs))) return QG_ERR_INVALID_ARG;
+    if (k > QG_LOGPROBS_MAX_TOP) return mfail(m, QG_ERR_SHAPE, "too many alternatives");
+    QGM_HIP(m, hipSetDevice(m->ctx->device));
+    const size_t vocab = m->cfg.vocab_size;
+    int rc;
+    if (!m->lp_work) {
+        const size_t held = m->allocs.size(), bytes = m->alloc_bytes;
+        if ((rc = qg_logprobs_work(m->ctx, 1, vocab, QG_LOGPROBS_MAX_TOP, &m->lp_work_bytes))) return rc;
+        if ((rc = dalloc(m, &m->lp_tok, kGiven)) || (rc = dalloc(m, &m->lp_out, kGiven)) ||
+            (rc = dalloc(m, &m->lp_ent, 1)) || (rc = dalloc(m, &m->lp_ids, QG_LOGPROBS_MAX_TOP)) ||
+            (rc = dalloc(m, &m->lp_top, QG_LOGPROBS_MAX_TOP)) ||
+            (rc = dalloc(m, &m->lp_work, m->lp_work_bytes + 16))) {
+            undo_allocs(m, held, bytes);
+            m->lp_tok = m->lp_ids = nullptr;
+            m->lp_out = m->lp_ent = m->lp_top = nullptr;
+            m->lp_work = nullptr;
+            return rc;
+        }
+    }
+    size_t at = 0;
+    do {
+        const size_t now = std::min<size_t>(n - at, kGiven), top = at ? 0 : k;
+        if (now) QGM_HIP(m, copy_wait(m, m->lp_tok, tokens + at, now * sizeof(uint32_t), hipMemcpyHostToDevice));
+        if ((rc = qg_logprobs_dev(m->ctx, m->logits, qg::T_F32, 1, vocab, vocab, m->lp_tok, now, m->lp_out,
+                                  entropy && !at ? m->lp_ent : nullptr, top, m->lp_ids, m->lp_top, m->lp_work,
+                                  m->lp_work_bytes, nullptr)))
+            return rc;
+        if (now) QGM_HIP(m, copy_wait(m, logprobs + at, m->lp_out, now * sizeof(float), hipMemcpyDeviceToHost));
+        if (top) {
+            QGM_HIP(m, copy_wait(m, top_ids, m->lp_ids, k * sizeof(uint32_t), hipMemcpyDeviceToHost));
+            QGM_HIP(m, copy_wait(m, top_logprobs, m->lp_top, k * sizeof(float), hipMemcpyDeviceToHost));
+        }
+        if (entropy && !at) QGM_HIP(m, copy_wait(m, entropy, m->lp_ent, sizeof(float), hipMemcpyDeviceToHost));
+        at += now;
+    } while (at < n);
     return QG_OK;
 }
 
