@@ -70,7 +70,7 @@ struct Problem {
     Rows q, out;
     uint32_t n_rep, rep_mul, rep_shift;    // x / n_rep = (mulhi(x, rep_mul) + x) >> rep_shift for x < 2^31
     uint32_t window;
-    uint32_t chunk;                        // blocks that are dealt out together
+    uint32_t chunk, lead;                  // blocks that are dealt out together; see width
     float scale2;      // |scale| log2(e)
     float sign;
     Work w;
@@ -111,6 +111,17 @@ template <uint32_t M> __device__ __forceinline__ Tile tile_of(const Problem &a, 
     return k;
 }
 
+// Lane l's sequence, to all.
+__device__ __forceinline__ Span span_at(const Span &s, uint32_t l)
+{
+    Span r;
+    r.row = (uint32_t)__builtin_amdgcn_readlane((int)s.row, (int)l);
+    r.n = (uint32_t)__builtin_amdgcn_readlane((int)s.n, (int)l);
+    r.len = (uint32_t)__builtin_amdgcn_readlane((int)s.len, (int)l);
+    r.pos = (int64_t)r.len - (int64_t)r.n;
+    return r;
+}
+
 // Sums over the lanes up to each (DPP: shifts within the rows of 16, then the
 // rows' last lanes to the rows behind them), and the last one's.
 template <int CTRL, int ROWS = 0xF> __device__ __forceinline__ uint32_t dpp0(uint32_t v)
@@ -132,62 +143,80 @@ __device__ __forceinline__ uint32_t lane_of(uint32_t v, uint32_t l)
     return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)l);
 }
 
-// Chunks of all tiles of a sequence (one kv head), by the whole wave.
-template <uint32_t M> __device__ uint32_t seq_chunks(const Problem &a, const Span &s)
+// What an item takes of the order: its chunks, and `lead` places before them
+// that stand for what every item costs whatever its length (its rows' way in and
+// out).
+__device__ __forceinline__ uint32_t width(const Problem &a, const Tile &t) { return t.chunks + a.lead; }
+
+// Places of all tiles of a sequence (one kv head), by the whole wave.
+template <uint32_t M> __device__ uint32_t seq_places(const Problem &a, const Span &s)
 {
     const uint32_t n = tiles_of<M>(a, s), lane = threadIdx.x & 63u;
     uint32_t c = 0;
-    for (uint32_t t = lane; t < n; t += 64) c += tile_of<M>(a, s, t).chunks;
+    for (uint32_t t = lane; t < n; t += 64) c += width(a, tile_of<M>(a, s, t));
     return lane_of(scan64(c), 63);
 }
 
-// Chunks of 64 sequences from s0 on, a sequence per lane, all kv heads.
-template <uint32_t M> __device__ uint32_t lane_chunks(const Problem &a, uint32_t s0)
+// Places of 64 sequences from s0 on, a sequence per lane, all kv heads; and the
+// lanes' sequences.
+template <uint32_t M> __device__ uint32_t lane_places(const Problem &a, uint32_t s0, Span *own)
 {
     const uint32_t lane = threadIdx.x & 63u, s = s0 + lane;
     uint32_t n = 0, c = 0;
+    *own = Span{};
     if (s < a.v.n_seqs) {
-        const Span p = span_of(a.b, s);
-        n = tiles_of<M>(a, p);
-        if (n == 1) c = tile_of<M>(a, p, 0).chunks;
+        *own = span_of(a.b, s);
+        n = tiles_of<M>(a, *own);
+        if (n == 1) c = width(a, tile_of<M>(a, *own, 0));
     }
     uint64_t many = __ballot(n > 1);
     while (many) {
         const uint32_t l = (uint32_t)__ffsll((unsigned long long)many) - 1;
         many &= many - 1;
-        const uint32_t t = seq_chunks<M>(a, span_of(a.b, s0 + l));
+        const uint32_t t = seq_places<M>(a, span_at(*own, l));
         if (lane == l) c = t;
     }
     return c * a.v.n_heads;
 }
 
+// The order: its length, the running sums and the sequences of the first 64.
+struct Order {
+    uint32_t total, first;
+    Span own;
+};
+
+template <uint32_t M> __device__ Order order_of(const Problem &a)
+{
+    Order o;
+    o.total = 0;
+    for (uint32_t s0 = 0; s0 < a.v.n_seqs; s0 += 64) {
+        Span own;
+        const uint32_t c = scan64(lane_places<M>(a, s0, &own));
+        if (s0 == 0) {
+            o.first = c;
+            o.own = own;
+        }
+        o.total += lane_of(c, 63);
+    }
+    return o;
+}
+
 struct Item {
-    uint32_t seq, head, tile;
-    uint32_t start;                     // chunk the item begins with
+    uint32_t seq, head, tile, tiles;
+    uint32_t start;                     // place of its first chunk
     Tile t;
     Span s;
 };
 
-// All sequences' chunks; `first` keeps the running sums of the first 64.
-template <uint32_t M> __device__ uint32_t all_chunks(const Problem &a, uint32_t *first)
-{
-    uint32_t total = 0;
-    for (uint32_t s0 = 0; s0 < a.v.n_seqs; s0 += 64) {
-        const uint32_t c = scan64(lane_chunks<M>(a, s0));
-        if (s0 == 0) *first = c;
-        total += lane_of(c, 63);
-    }
-    return total;
-}
-
-// The item that holds chunk `at` (less than the total).
-template <uint32_t M> __device__ Item find(const Problem &a, uint32_t at, uint32_t first)
+// The item that holds place `at` (less than the total).
+template <uint32_t M> __device__ Item find(const Problem &a, uint32_t at, const Order &o)
 {
     const uint32_t lane = threadIdx.x & 63u;
     Item it{};
     uint32_t before = 0;
     for (uint32_t s0 = 0; s0 < a.v.n_seqs; s0 += 64) {
-        const uint32_t c = s0 == 0 ? first : scan64(lane_chunks<M>(a, s0));
+        Span own = o.own;
+        const uint32_t c = s0 == 0 ? o.first : scan64(lane_places<M>(a, s0, &own));
         const uint64_t past = __ballot(before + c > at);
         if (!past) {
             before += lane_of(c, 63);
@@ -196,14 +225,15 @@ template <uint32_t M> __device__ Item find(const Problem &a, uint32_t at, uint32
         const uint32_t l = (uint32_t)__ffsll((unsigned long long)past) - 1;
         const uint32_t up_to = lane_of(c, l), below = l ? lane_of(c, l - 1) : 0u;
         it.seq = s0 + l;
-        it.s = span_of(a.b, it.seq);
+        it.s = span_at(own, l);
         before += below;
         const uint32_t per_head = (up_to - below) / a.v.n_heads;
         it.head = (at - before) / per_head;
         before += it.head * per_head;
-        const uint32_t n = tiles_of<M>(a, it.s);
-        for (uint32_t t0 = 0; t0 < n; t0 += 64) {
-            const uint32_t d = n == 1 ? per_head : scan64(t0 + lane < n ? tile_of<M>(a, it.s, t0 + lane).chunks : 0u);
+        it.tiles = tiles_of<M>(a, it.s);
+        for (uint32_t t0 = 0; t0 < it.tiles; t0 += 64) {
+            const uint32_t d = it.tiles == 1 ? per_head
+                               : scan64(t0 + lane < it.tiles ? width(a, tile_of<M>(a, it.s, t0 + lane)) : 0u);
             const uint64_t in = __ballot(before + d > at);
             if (!in) {
                 before += lane_of(d, 63);
@@ -211,13 +241,30 @@ template <uint32_t M> __device__ Item find(const Problem &a, uint32_t at, uint32
             }
             const uint32_t k = (uint32_t)__ffsll((unsigned long long)in) - 1;
             it.tile = t0 + k;
-            it.start = before + (k ? lane_of(d, k - 1) : 0u);
+            it.start = before + (k ? lane_of(d, k - 1) : 0u) + a.lead;
             it.t = tile_of<M>(a, it.s, it.tile);
             return it;
         }
         return it;
     }
     return it;
+}
+
+// The item behind `it`: the next tile, else the next head, else the next sequence.
+template <uint32_t M> __device__ void advance(const Problem &a, Item &it, const Order &o)
+{
+    const uint32_t end = it.start + it.t.chunks;
+    if (it.tile + 1 < it.tiles) {
+        it.tile++;
+    } else if (it.head + 1 < a.v.n_heads) {
+        it.head++;
+        it.tile = 0;
+    } else {
+        it = find<M>(a, end, o);
+        return;
+    }
+    it.start = end + a.lead;
+    it.t = tile_of<M>(a, it.s, it.tile);
 }
 
 // Eight codes (bytes code + 128) as f16: 1024 + byte by its bits, less 1152.
@@ -246,37 +293,30 @@ template <int DP, int NP> struct QFrag {
     float f;                  // s = f * (key scale) * acc
 };
 
-// at < 0: no row
-template <int DP, int NP>
-__device__ void load_q(const Problem &a, bool valid, uint64_t at, uint32_t g, QFrag<DP, NP> &q)
+// x: the lane's elements 64 c' + 16 g + 4 c'' .. + 4 at 4 c' + c''
+template <int DP, int NP> __device__ __forceinline__ void load_q(const Problem &a, const float4 *x, QFrag<DP, NP> &q)
 {
-    float x[DP / 64][16];
     uint32_t m = 0;
 #pragma unroll
-    for (int c = 0; c < DP / 64; c++) {
-        if (valid) {
-            load16(a.q, at, 64u * c + 16u * g, a.v.hd, x[c]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; j++) x[c][j] = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 16; j++) m = max(m, __float_as_uint(x[c][j]) & 0x7FFFFFFFu);
+    for (int c = 0; c < DP / 16; c++) {
+        m = max(max(m, __float_as_uint(x[c].x) & 0x7FFFFFFFu), __float_as_uint(x[c].y) & 0x7FFFFFFFu);
+        m = max(max(m, __float_as_uint(x[c].z) & 0x7FFFFFFFu), __float_as_uint(x[c].w) & 0x7FFFFFFFu);
     }
     m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
     m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
     // largest magnitude into [1024, 2048): 2^up, within what keeps 2^-up and q 2^up normal
-    const int up = m >= 0x7F800000u ? 0 : min(137 - (int)(m >> 23), 110);
+    const bool bad = m >= 0x7F800000u;
+    const int up = bad ? 0 : min(137 - (int)(m >> 23), 110);
     const float s = ldexpf(a.sign, up);
-    q.f = m >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : ldexpf(a.scale2, -up);
+    q.f = bad ? __uint_as_float(0x7FC00000u) : ldexpf(a.scale2, -up);
 #pragma unroll
-    for (int c = 0; c < DP / 64; c++)
+    for (int c = 0; c < DP / 16; c++)
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const float y = m >= 0x7F800000u ? 0.f : x[c][j] * s;
+        for (int j = 0; j < 4; j++) {
+            const float y = bad ? 0.f : (j == 0 ? x[c].x : j == 1 ? x[c].y : j == 2 ? x[c].z : x[c].w) * s;
             const _Float16 hi = (_Float16)y;
-            q.h[0][2 * c + j / 8][j % 8] = hi;
-            if (NP == 2) q.h[NP - 1][2 * c + j / 8][j % 8] = (_Float16)(y - (float)hi);
+            q.h[0][c / 2][c % 2 * 4 + j] = hi;
+            if (NP == 2) q.h[NP - 1][c / 2][c % 2 * 4 + j] = (_Float16)(y - (float)hi);
         }
 }
 
@@ -423,22 +463,68 @@ template <uint32_t M> __device__ __forceinline__ Row row_of(const Problem &a, co
     return w;
 }
 
-// n consecutive elements of an output row (n a multiple of 4, d too)
-__device__ __forceinline__ void store_row(const Rows &o, uint64_t at, uint32_t d, uint32_t hd, const float *x, int n)
+// Elements d .. d + 4 of a row (d a multiple of 4).
+__device__ __forceinline__ void store4v(const Rows &r, uint64_t at, uint32_t d, uint32_t hd, float4 x)
 {
-    if (o.vec && d + (uint32_t)n <= hd) {
-        for (int i = 0; i < n; i += 4) {
-            if (o.f16) {
-                typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-                *(h4 *)((_Float16 *)o.p + at + d + i) = h4{(_Float16)x[i], (_Float16)x[i + 1], (_Float16)x[i + 2], (_Float16)x[i + 3]};
-            } else {
-                *(float4 *)((float *)o.p + at + d + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    if (d >= hd) return;
+    if (r.f16) *(h4 *)((_Float16 *)r.p + at + d) = h4{(_Float16)x.x, (_Float16)x.y, (_Float16)x.z, (_Float16)x.w};
+    else *(float4 *)((float *)r.p + at + d) = x;
+}
+__device__ __forceinline__ void store4(const Rows &r, uint64_t at, uint32_t d, uint32_t hd, float4 x)
+{
+    if (r.vec) {
+        store4v(r, at, d, hd, x);
+        return;
+    }
+    if (d < hd) store1(r, at + d, x.x);
+    if (d + 1 < hd) store1(r, at + d + 1, x.y);
+    if (d + 2 < hd) store1(r, at + d + 2, x.z);
+    if (d + 3 < hd) store1(r, at + d + 3, x.w);
+}
+
+// What a wave's lanes have written to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A wave's 16 rows r0 .. of a tile's q (`row` the lane's) as load_q takes them:
+// straight from memory, or, where the rows take no 16-byte accesses, element by
+// element through LDS (rows of DP + 4 floats at `to`).
+template <uint32_t M, int DP>
+__device__ __forceinline__ void take_q(const Problem &a, const Item &it, uint32_t r0, const Row &row, float *to, float4 *x)
+{
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
+    if (a.q.vec) {
+        const uint64_t at = row.row * a.q.ld_row + row.head * a.q.ld_head;
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++) {
+            const uint32_t d = 64 * (c / 4) + 16 * g + 4 * (c % 4);
+            x[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row.valid && d < a.v.hd) {
+                if (a.q.f16) {
+                    const h4 h = *(const h4 *)((const _Float16 *)a.q.p + at + d);
+                    x[c] = make_float4((float)h[0], (float)h[1], (float)h[2], (float)h[3]);
+                } else {
+                    x[c] = *(const float4 *)((const float *)a.q.p + at + d);
+                }
             }
         }
-    } else {
-        for (int i = 0; i < n; i++)
-            if (d + i < hd) store1(o, at + d + i, x[i]);
+        return;
     }
+#pragma unroll 1
+    for (uint32_t u = lane; u < 16u * DP; u += 64) {
+        const uint32_t k = u / DP, d = u % DP;
+        const Row w = row_of<M>(a, it.s, it.head, it.tile, r0 + k);
+        to[k * (DP + 4) + d] = w.valid && d < a.v.hd ? load1(a.q, w.row * a.q.ld_row + w.head * a.q.ld_head + d) : 0.f;
+    }
+    wave_sync();
+#pragma unroll
+    for (int c = 0; c < DP / 16; c++) x[c] = *(const float4 *)(to + r * (DP + 4) + 64 * (c / 4) + 16 * g + 4 * (c % 4));
+    wave_sync();
 }
 
 template <uint32_t M> __device__ __forceinline__ void put_split(const Problem &a, uint32_t wg, const Item *it, uint32_t per)
@@ -473,27 +559,23 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
 {
     constexpr int NK = DP / 32, NV = DP / 32;             // 16-byte loads of a lane per block
     constexpr int LD = DP + 4;
-    __shared__ float so[4][16][LD], sm[4][16], sl[4][16];
+    __shared__ __attribute__((aligned(16))) float so[4][16][LD], sm[4][16], sl[4][16];
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
     const uint32_t wg = place_of(blockIdx.x, gridDim.x);
-    uint32_t first;
-    const uint32_t total = all_chunks<kFewM>(a, &first);
-    const uint32_t per = (total + gridDim.x - 1) / gridDim.x;
+    const Order order = order_of<kFewM>(a);
+    const uint32_t per = (order.total + gridDim.x - 1) / gridDim.x;
     uint32_t at = wg * per;
-    const uint32_t end = min(at + per, total);
+    const uint32_t end = min(at + per, order.total);
     if (at >= end) {
         put_split<kFewM>(a, wg, nullptr, per);
         return;
     }
-    bool begun = false;
+    Item it = find<kFewM>(a, at, order);
+    put_split<kFewM>(a, wg, at > it.start ? &it : nullptr, per);
     const uint64_t all = (uint64_t)a.v.n_seqs * a.v.n_heads;
-    while (at < end) {
-        const Item it = find<kFewM>(a, at, first);
-        const uint32_t c0 = at - it.start, nc = min(it.t.chunks - c0, end - at);
-        if (!begun) {
-            put_split<kFewM>(a, wg, c0 ? &it : nullptr, per);
-            begun = true;
-        }
+    for (;;) {
+        if (it.start >= end) break;                      // only its lead is here
+        const uint32_t c0 = at > it.start ? at - it.start : 0u, nc = min(it.t.chunks, end - it.start) - c0;
         const uint64_t sh = (uint64_t)it.seq * a.v.n_heads + it.head;
         const uint8_t *kb = a.v.codes + sh * a.v.n_blocks * (kBlock * DP) + lane * 16u;
         const uint8_t *vb = a.v.codes + (all + sh) * a.v.n_blocks * (kBlock * DP) + lane * 16u;
@@ -512,10 +594,13 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
             ksc = ks[b];
             vsc = vs[b];
         };
-        if (blk < last) fetch(blk);
         const Row row = row_of<kFewM>(a, it.s, it.head, it.tile, r);
+        if (!a.q.vec) __syncthreads();            // the part before is done with so
+        float4 qx[DP / 16];
+        take_q<kFewM, DP>(a, it, 0, row, &so[wave][0][0], qx);
+        if (blk < last) fetch(blk);
         QFrag<DP, NP> q;
-        load_q<DP, NP>(a, row.valid, row.row * a.q.ld_row + row.head * a.q.ld_head, g, q);
+        load_q<DP, NP>(a, qx, q);
         const int32_t lo = from(row.lo, (int64_t)blk0 * kBlock), hi = from(row.hi, (int64_t)blk0 * kBlock);
         State<DP> st;
         st.m = kLow;
@@ -596,30 +681,31 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
         for (uint32_t u = threadIdx.x; u < 16u * (DP / 4); u += 256) {
             const uint32_t rr = u / (DP / 4), d = u % (DP / 4) * 4u;
             const float m = fmaxf(fmaxf(sm[0][rr], sm[1][rr]), fmaxf(sm[2][rr], sm[3][rr]));
-            float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+            float l = 0.f;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < 4; w++) {
                 const float e = exp2_(sm[w][rr] - m);
                 l += e * sl[w][rr];
                 const float4 o = *(const float4 *)&so[w][rr][d];
-                x[0] += e * o.x; x[1] += e * o.y; x[2] += e * o.z; x[3] += e * o.w;
+                x.x += e * o.x; x.y += e * o.y; x.z += e * o.z; x.w += e * o.w;
             }
             if (whole) {
                 const Row w = row_of<kFewM>(a, it.s, it.head, it.tile, rr);
                 if (!w.valid) continue;
-                const float inv = w.hi > w.lo ? 1.f / l : 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[i] = w.hi > w.lo ? x[i] * inv : 0.f;
-                store_row(a.out, w.row * a.out.ld_row + w.head * a.out.ld_head, d, a.v.hd, x, 4);
+                const float inv = 1.f / l;
+                x = w.hi > w.lo ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
+                store4(a.out, w.row * a.out.ld_row + w.head * a.out.ld_head, d, a.v.hd, x);
             } else {
-                *(float4 *)(a.w.part + (slot * kFewM + rr) * DP + d) = make_float4(x[0], x[1], x[2], x[3]);
+                *(float4 *)(a.w.part + (slot * kFewM + rr) * DP + d) = x;
                 if (d == 0) {
                     a.w.ml[(slot * kFewM + rr) * 2] = m;
                     a.w.ml[(slot * kFewM + rr) * 2 + 1] = l;
                 }
             }
         }
-        at += nc;
+        if (it.start + it.t.chunks >= end) break;
+        advance<kFewM>(a, it, order);
     }
 }
 
@@ -638,25 +724,22 @@ template <int DP, int NP, int RT> __global__ void __launch_bounds__(256, 2) many
     extern __shared__ __attribute__((aligned(16))) h8 stage[];        // [3][keys, values][DP / 32 * 2][64]
     constexpr uint32_t kOne = DP * 4;                                 // operands of 16 bytes: keys or values of a block
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
+    float *const mine = (float *)(stage + wave * (kOne * 3 / 2));        // 16 rows of DP + 4 floats fit
     const uint32_t wg = place_of(blockIdx.x, gridDim.x);
-    uint32_t first;
-    const uint32_t total = all_chunks<M>(a, &first);
-    const uint32_t per = (total + gridDim.x - 1) / gridDim.x;
+    const Order order = order_of<M>(a);
+    const uint32_t per = (order.total + gridDim.x - 1) / gridDim.x;
     uint32_t at = wg * per;
-    const uint32_t end = min(at + per, total);
+    const uint32_t end = min(at + per, order.total);
     if (at >= end) {
         put_split<M>(a, wg, nullptr, per);
         return;
     }
-    bool begun = false;
+    Item it = find<M>(a, at, order);
+    put_split<M>(a, wg, at > it.start ? &it : nullptr, per);
     const uint64_t all = (uint64_t)a.v.n_seqs * a.v.n_heads;
-    while (at < end) {
-        const Item it = find<M>(a, at, first);
-        const uint32_t c0 = at - it.start, nc = min(it.t.chunks - c0, end - at);
-        if (!begun) {
-            put_split<M>(a, wg, c0 ? &it : nullptr, per);
-            begun = true;
-        }
+    for (;;) {
+        if (it.start >= end) break;                      // only its lead is here
+        const uint32_t c0 = at > it.start ? at - it.start : 0u, nc = min(it.t.chunks, end - it.start) - c0;
         const uint64_t sh = (uint64_t)it.seq * a.v.n_heads + it.head;
         // the part's first block; n of them (0: an item that sees nothing)
         const uint32_t blk0 = it.t.blk0 + c0 * a.chunk;
@@ -674,22 +757,37 @@ template <int DP, int NP, int RT> __global__ void __launch_bounds__(256, 2) many
                 code[i] = *(const uint4 *)(u < 2 * DP ? kb + off + u * 16u : vb + off + (u - 2 * DP) * 16u);
             }
         };
-        auto put = [&](uint32_t slot, int half) {         // half: of 2 NU
+        auto put = [&](uint32_t slot, int half, uint4 w) {        // half: of 2 NU
             const uint32_t u = threadIdx.x + 256u * (half / 2);
             h8 *to = stage + slot * 2 * kOne + (u >> 6) * 128u + lane + half % 2 * 64;
-            const uint4 w = code[half / 2];
             *to = half % 2 ? halves(w.z, w.w) : halves(w.x, w.y);
         };
-        if (n) fetch(0);
+        Row row[RT];
+        float4 qx[RT][DP / 16];
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            row[t] = row_of<M>(a, it.s, it.head, it.tile, (wave * RT + t) * 16u + r);
+            // LDS: the wave's quarter of the ring (every part ends with a barrier)
+            take_q<M, DP>(a, it, (wave * RT + t) * 16u, row[t], mine, qx[t]);
+        }
+        uint4 code0[NU], code1[NU];
+        if (n) {
+            fetch(0);
+#pragma unroll
+            for (int i = 0; i < NU; i++) code0[i] = code[i];
+            fetch(1);
+#pragma unroll
+            for (int i = 0; i < NU; i++) code1[i] = code[i];
+            fetch(2);
+        }
         QFrag<DP, NP> q[RT];
         State<DP> st[RT];
         int32_t lo[RT], hi[RT], lo_all = 0, hi_all = 0x7FFFFFFF;
 #pragma unroll
         for (int t = 0; t < RT; t++) {
-            const Row row = row_of<M>(a, it.s, it.head, it.tile, (wave * RT + t) * 16u + r);
-            load_q<DP, NP>(a, row.valid, row.row * a.q.ld_row + row.head * a.q.ld_head, g, q[t]);
-            lo[t] = from(row.lo, (int64_t)blk0 * kBlock);
-            hi[t] = from(row.hi, (int64_t)blk0 * kBlock);
+            load_q<DP, NP>(a, qx[t], q[t]);
+            lo[t] = from(row[t].lo, (int64_t)blk0 * kBlock);
+            hi[t] = from(row[t].hi, (int64_t)blk0 * kBlock);
             lo_all = max(lo_all, lo[t]);
             hi_all = min(hi_all, hi[t]);
             st[t].m = kLow;
@@ -786,7 +884,7 @@ template <int DP, int NP, int RT> __global__ void __launch_bounds__(256, 2) many
                 for (int t = 0; t < RT; t++)
 #pragma unroll
                     for (int k = 0; k < NP; k++) st[t].o[i] = mfma(w, p[t][k], st[t].o[i]);
-                if (i % 2) put(s2, i / 2);                // block j + 2, where j - 1 was
+                if (i % 2) put(s2, i / 2, code[i / 4]);   // block j + 2, where j - 1 was
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
@@ -797,11 +895,10 @@ template <int DP, int NP, int RT> __global__ void __launch_bounds__(256, 2) many
         if (n) {
             __syncthreads();                              // the part before is done with the ring
 #pragma unroll
-            for (int i = 0; i < 2 * NU; i++) put(0, i);
-            fetch(1);
-#pragma unroll
-            for (int i = 0; i < 2 * NU; i++) put(1, i);
-            fetch(2);
+            for (int i = 0; i < 2 * NU; i++) {
+                put(0, i, code0[i / 2]);
+                put(1, i, code1[i / 2]);
+            }
             ksn = ks[0];
             vsn = vs[0];
             __syncthreads();
@@ -825,31 +922,44 @@ template <int DP, int NP, int RT> __global__ void __launch_bounds__(256, 2) many
             float l = st[t].l;
             l += __shfl_xor(l, 16, 64);
             l += __shfl_xor(l, 32, 64);
-            const Row w = row_of<M>(a, it.s, it.head, it.tile, rr);
-            const float k = !whole ? ref.ref : w.hi > w.lo ? ref.ref / l : 0.f;
+            const float k = whole ? ref.ref / l : ref.ref;
             if (!whole && g == 0) {
                 a.w.ml[(slot * M + rr) * 2] = st[t].m;
                 a.w.ml[(slot * M + rr) * 2 + 1] = l;
             }
+            // lane (r, g) holds elements 32 i + 8 g .. + 8 of row r
+            const Row w = row_of<M>(a, it.s, it.head, it.tile, rr);
+            const uint64_t to = w.row * a.out.ld_row + w.head * a.out.ld_head;
+            float *const part = a.w.part + (slot * M + rr) * DP;
+            const bool sees = !whole || w.hi > w.lo, direct = !whole || a.out.vec;
 #pragma unroll
             for (int i = 0; i < DP / 32; i++) {
-                float x[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    x[j] = st[t].o[2 * i + (j & 1)][j >> 1] * k;
-                    if (whole && !(w.hi > w.lo)) x[j] = 0.f;
-                }
-                const uint32_t d = 32 * i + 8 * g;
-                if (!whole) {
-                    float4 *o = (float4 *)(a.w.part + (slot * M + rr) * DP + d);
-                    o[0] = make_float4(x[0], x[1], x[2], x[3]);
-                    o[1] = make_float4(x[4], x[5], x[6], x[7]);
-                } else if (w.valid) {
-                    store_row(a.out, w.row * a.out.ld_row + w.head * a.out.ld_head, d, a.v.hd, x, 8);
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t d = 32 * i + 8 * g + 4 * h;
+                    float4 x = make_float4(st[t].o[2 * i][2 * h] * k, st[t].o[2 * i + 1][2 * h] * k,
+                                           st[t].o[2 * i][2 * h + 1] * k, st[t].o[2 * i + 1][2 * h + 1] * k);
+                    if (!sees) x = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (!whole) *(float4 *)(part + d) = x;
+                    else if (!direct) *(float4 *)(mine + r * (DP + 4) + d) = x;
+                    else if (w.valid) store4v(a.out, to, d, a.v.hd, x);
                 }
             }
+            if (!direct) {                                // element by element, through LDS
+                wave_sync();
+#pragma unroll 1
+                for (uint32_t u = lane; u < 16u * DP; u += 64) {
+                    const uint32_t x = u / DP, d = u % DP;
+                    const Row y = row_of<M>(a, it.s, it.head, it.tile, (wave * RT + t) * 16u + x);
+                    if (y.valid && d < a.v.hd)
+                        store1(a.out, y.row * a.out.ld_row + y.head * a.out.ld_head + d, mine[x * (DP + 4) + d]);
+                }
+                wave_sync();
+            }
         }
-        at += nc;
+        if (!n) __syncthreads();                          // as every part ends
+        if (it.start + it.t.chunks >= end) break;
+        advance<M>(a, it, order);
     }
 }
 
@@ -895,9 +1005,8 @@ template <uint32_t M, int DP, bool PARTS> __global__ void __launch_bounds__(256)
         const Row w = row_of<M>(a, span, s.head, s.tile, r);
         if (!w.valid) continue;
         const float inv = 1.f / l;
-        float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
-        if (!(w.hi > w.lo)) y[0] = y[1] = y[2] = y[3] = 0.f;
-        store_row(a.out, w.row * a.out.ld_row + w.head * a.out.ld_head, d, a.v.hd, y, 4);
+        x = w.hi > w.lo ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
+        store4(a.out, w.row * a.out.ld_row + w.head * a.out.ld_head, d, a.v.hd, x);
     }
 }
 
@@ -998,8 +1107,9 @@ int launch_attention(const View &v, const Batch &b, uint32_t n_heads, const Rows
     // a block for each wave of few_k, two of many_k; more where the chunks
     // would not be counted in 31 bits (all tiles seeing the whole cache)
     a.chunk = kind == kFew ? 4u : 2u;
+    a.lead = kind == kFew ? 0u : 4u;
     const uint64_t tiles = ((uint64_t)b.n_rows * a.n_rep + tile_rows(kind) - 1) / tile_rows(kind) + v.n_seqs;
-    while (tiles * v.n_heads * (v.n_blocks / a.chunk + 1) >> 31) a.chunk *= 2;
+    while (tiles * v.n_heads * (v.n_blocks / a.chunk + 1 + a.lead) >> 31) a.chunk *= 2;
     a.w = work_at(work, workgroups(n_cu), tile_rows(kind));
     switch (v.dp) {
     case 64: return launch_dp<64>(a, kind, n_cu, st);
