@@ -496,21 +496,26 @@ __device__ __forceinline__ void wave_sync()
 template <uint32_t M, int DP>
 __device__ __forceinline__ void take_q(const Problem &a, const Item &it, uint32_t r0, const Row &row, float *to, float4 *x)
 {
-    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
     const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
     if (a.q.vec) {
         const uint64_t at = row.row * a.q.ld_row + row.head * a.q.ld_head;
 #pragma unroll
-        for (int c = 0; c < DP / 16; c++) {
-            const uint32_t d = 64 * (c / 4) + 16 * g + 4 * (c % 4);
-            x[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (row.valid && d < a.v.hd) {
-                if (a.q.f16) {
-                    const h4 h = *(const h4 *)((const _Float16 *)a.q.p + at + d);
-                    x[c] = make_float4((float)h[0], (float)h[1], (float)h[2], (float)h[3]);
-                } else {
-                    x[c] = *(const float4 *)((const float *)a.q.p + at + d);
-                }
+        for (int c = 0; c < DP / 16; c++) x[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!row.valid) return;
+        if (a.q.f16) {
+#pragma unroll
+            for (int c = 0; c < DP / 16; c += 2) {
+                const uint32_t d = 64 * (c / 4) + 16 * g + 4 * (c % 4);
+                if (d >= a.v.hd) continue;
+                const h8 h = *(const h8 *)((const _Float16 *)a.q.p + at + d);
+                x[c] = make_float4((float)h[0], (float)h[1], (float)h[2], (float)h[3]);
+                x[c + 1] = make_float4((float)h[4], (float)h[5], (float)h[6], (float)h[7]);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < DP / 16; c++) {
+                const uint32_t d = 64 * (c / 4) + 16 * g + 4 * (c % 4);
+                if (d < a.v.hd) x[c] = *(const float4 *)((const float *)a.q.p + at + d);
             }
         }
         return;
@@ -572,33 +577,52 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
     }
     Item it = find<kFewM>(a, at, order);
     put_split<kFewM>(a, wg, at > it.start ? &it : nullptr, per);
+    if (it.start >= end) return;                             // only its lead is here
     const uint64_t all = (uint64_t)a.v.n_seqs * a.v.n_heads;
-    for (;;) {
-        if (it.start >= end) break;                      // only its lead is here
-        const uint32_t c0 = at > it.start ? at - it.start : 0u, nc = min(it.t.chunks, end - it.start) - c0;
+    const uint8_t *kb, *vb;
+    const float *ks, *vs;
+    uint32_t c0, nc, blk0, last, blk;
+    uint4 k[NK], v[NV];
+    float ksc = 0.f, vsc = 0.f;
+    Row row;
+    float4 qx[DP / 16];
+    auto fetch_k = [&](uint32_t b) {
+        const uint64_t off = (uint64_t)b * (kBlock * DP);
+#pragma unroll
+        for (int i = 0; i < NK; i++) k[i] = *(const uint4 *)(kb + off + i * 1024);
+        ksc = ks[b];
+    };
+    auto fetch_v = [&](uint32_t b) {
+        const uint64_t off = (uint64_t)b * (kBlock * DP);
+#pragma unroll
+        for (int i = 0; i < NV; i++) v[i] = *(const uint4 *)(vb + off + i * 1024);
+        vsc = vs[b];
+    };
+    // the part of `it` that is here, and its first loads
+    auto begin = [&]() {
+        c0 = at > it.start ? at - it.start : 0u;
+        nc = min(it.t.chunks, end - it.start) - c0;
         const uint64_t sh = (uint64_t)it.seq * a.v.n_heads + it.head;
-        const uint8_t *kb = a.v.codes + sh * a.v.n_blocks * (kBlock * DP) + lane * 16u;
-        const uint8_t *vb = a.v.codes + (all + sh) * a.v.n_blocks * (kBlock * DP) + lane * 16u;
-        const float *ks = a.v.scale + sh * a.v.n_blocks, *vs = a.v.scale + (all + sh) * a.v.n_blocks;
-        const uint32_t last = it.t.blk0 + min(it.t.blocks, (c0 + nc) * a.chunk);
-        const uint32_t blk0 = it.t.blk0 + c0 * a.chunk;
-        uint32_t blk = blk0 + wave;
-        uint4 k[NK], v[NV];
-        float ksc = 0.f, vsc = 0.f;
-        auto fetch = [&](uint32_t b) {
-            const uint64_t off = (uint64_t)b * (kBlock * DP);
-#pragma unroll
-            for (int i = 0; i < NK; i++) k[i] = *(const uint4 *)(kb + off + i * 1024);
-#pragma unroll
-            for (int i = 0; i < NV; i++) v[i] = *(const uint4 *)(vb + off + i * 1024);
-            ksc = ks[b];
-            vsc = vs[b];
-        };
-        const Row row = row_of<kFewM>(a, it.s, it.head, it.tile, r);
-        if (!a.q.vec) __syncthreads();            // the part before is done with so
-        float4 qx[DP / 16];
-        take_q<kFewM, DP>(a, it, 0, row, &so[wave][0][0], qx);
-        if (blk < last) fetch(blk);
+        kb = a.v.codes + sh * a.v.n_blocks * (kBlock * DP) + lane * 16u;
+        vb = a.v.codes + (all + sh) * a.v.n_blocks * (kBlock * DP) + lane * 16u;
+        ks = a.v.scale + sh * a.v.n_blocks;
+        vs = a.v.scale + (all + sh) * a.v.n_blocks;
+        last = it.t.blk0 + min(it.t.blocks, (c0 + nc) * a.chunk);
+        blk0 = it.t.blk0 + c0 * a.chunk;
+        blk = blk0 + wave;
+        row = row_of<kFewM>(a, it.s, it.head, it.tile, r);
+        if (blk < last) {
+            fetch_k(blk);
+            fetch_v(blk);
+        }
+        if (a.q.vec) take_q<kFewM, DP>(a, it, 0, row, nullptr, qx);
+    };
+    begin();
+    for (;;) {
+        if (!a.q.vec) {
+            __syncthreads();                      // the part before is done with so
+            take_q<kFewM, DP>(a, it, 0, row, &so[wave][0][0], qx);
+        }
         QFrag<DP, NP> q;
         load_q<DP, NP>(a, qx, q);
         const int32_t lo = from(row.lo, (int64_t)blk0 * kBlock), hi = from(row.hi, (int64_t)blk0 * kBlock);
@@ -609,19 +633,16 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
         for (int i = 0; i < DP / 16; i++) st.o[i] = v4f{0.f, 0.f, 0.f, 0.f};
         Ref ref{0.f, 0.f};
         while (blk < last) {
-            uint4 kc[NK], vc[NV];
-#pragma unroll
-            for (int i = 0; i < NK; i++) kc[i] = k[i];
-#pragma unroll
-            for (int i = 0; i < NV; i++) vc[i] = v[i];
-            const float kcs = ksc, vcs = vsc;
-            if (blk + 4 < last) fetch(blk + 4);
+            // the next block's loads are in flight while a block is worked on: its
+            // keys' from where these are used up, its values' likewise
+            const float kcs = ksc;
+            const bool more = blk + 4 < last;
             v4f acc[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int c = 0; c < DP / 64; c++)
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
-                    const uint4 w = kc[t * (DP / 64) + c];
+                    const uint4 w = k[t * (DP / 64) + c];
                     const h8 x = halves(w.x, w.y), y = halves(w.z, w.w);
 #pragma unroll
                     for (int n = 0; n < NP; n++) {
@@ -629,6 +650,8 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
                         acc[t] = mfma(y, q.h[n][2 * c + 1], acc[t]);
                     }
                 }
+            if (more) fetch_k(blk + 4);
+            const float vcs = vsc;
             float log, inv;
             refer<DP, 1>(vcs, ref, &st);
             ratio_of(vcs, ref, &log, &inv);
@@ -646,16 +669,26 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
             st.l = __builtin_fmaf(sum, inv, st.l);
 #pragma unroll
             for (int i = 0; i < DP / 32; i++) {
-                const h8 x = halves(vc[i].x, vc[i].y), y = halves(vc[i].z, vc[i].w);
+                const h8 x = halves(v[i].x, v[i].y), y = halves(v[i].z, v[i].w);
 #pragma unroll
                 for (int n = 0; n < NP; n++) {
                     st.o[2 * i] = mfma(x, p[n], st.o[2 * i]);
                     st.o[2 * i + 1] = mfma(y, p[n], st.o[2 * i + 1]);
                 }
             }
+            if (more) fetch_v(blk + 4);
             blk += 4;
         }
-        // join the waves: lane (r, g) holds elements 32 i + 8 g .. + 8 of row r
+        // the next part's loads are in flight while this one's waves are joined
+        const Item done = it;
+        const bool from0 = c0 == 0, whole = from0 && nc == it.t.chunks;
+        bool go = it.start + it.t.chunks < end;
+        if (go) {
+            advance<kFewM>(a, it, order);
+            go = it.start < end;
+            if (go) begin();
+        }
+        // lane (r, g) holds elements 32 i + 8 g .. + 8 of row r
         st.l += __shfl_xor(st.l, 16, 64);
         st.l += __shfl_xor(st.l, 32, 64);
         __syncthreads();
@@ -676,8 +709,7 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
             }
         }
         __syncthreads();
-        const bool whole = c0 == 0 && nc == it.t.chunks;
-        const uint64_t slot = (uint64_t)wg * 2 + (c0 ? 0u : 1u);
+        const uint64_t slot = (uint64_t)wg * 2 + (from0 ? 1u : 0u);
         for (uint32_t u = threadIdx.x; u < 16u * (DP / 4); u += 256) {
             const uint32_t rr = u / (DP / 4), d = u % (DP / 4) * 4u;
             const float m = fmaxf(fmaxf(sm[0][rr], sm[1][rr]), fmaxf(sm[2][rr], sm[3][rr]));
@@ -691,7 +723,7 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
                 x.x += e * o.x; x.y += e * o.y; x.z += e * o.z; x.w += e * o.w;
             }
             if (whole) {
-                const Row w = row_of<kFewM>(a, it.s, it.head, it.tile, rr);
+                const Row w = row_of<kFewM>(a, done.s, done.head, done.tile, rr);
                 if (!w.valid) continue;
                 const float inv = 1.f / l;
                 x = w.hi > w.lo ? make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -704,8 +736,7 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
                 }
             }
         }
-        if (it.start + it.t.chunks >= end) break;
-        advance<kFewM>(a, it, order);
+        if (!go) break;
     }
 }
 
@@ -1035,11 +1066,16 @@ Work work_at(void *p, uint32_t wgs, uint32_t m)
 // tiles read and convert the cache less often.
 enum Kind { kFew, kMany64, kMany128 };
 
-Kind kind_of(const View &v, uint64_t n_rows, bool starts, uint64_t n_rep)
+Kind kind_of(const View &v, uint64_t n_rows, bool starts, uint64_t n_rep, int n_cu)
 {
     const uint64_t pairs = starts ? n_rows * n_rep / std::min<uint64_t>(v.n_seqs, n_rows ? n_rows : 1) : n_rep;
     if (pairs <= 32) return kFew;
-    return pairs <= 64 || v.dp > 128 ? kMany64 : kMany128;
+    // tiles of 128 pairs where there are enough of them for the workgroups: with
+    // fewer, the items are cut anyway, and the smaller ones have less to begin and
+    // end with (1001 tokens of 32 heads 44.6 against 54.4 us, f32; 5000 of them over
+    // four sequences 597 against 452, f16)
+    const uint64_t tiles = (n_rows * n_rep + 127) / 128 * v.n_heads;
+    return pairs <= 64 || v.dp > 128 || tiles < workgroups(n_cu) ? kMany64 : kMany128;
 }
 
 uint32_t tile_rows(Kind k)
@@ -1083,8 +1119,8 @@ template <int DP> int launch_dp(Problem &a, Kind kind, int n_cu, hipStream_t st)
 size_t attention_work(const View &v, size_t n_rows, size_t n_heads, int n_cu)
 {
     // calls of fewer rows take no larger tiles
-    const uint32_t m = std::max(tile_rows(kind_of(v, n_rows, true, n_heads / v.n_heads)),
-                                tile_rows(kind_of(v, n_rows, false, n_heads / v.n_heads)));
+    const uint32_t m = std::max(tile_rows(kind_of(v, n_rows, true, n_heads / v.n_heads, n_cu)),
+                                tile_rows(kind_of(v, n_rows, false, n_heads / v.n_heads, n_cu)));
     return work_bytes(workgroups(n_cu), m, v.dp);
 }
 
@@ -1101,13 +1137,15 @@ int launch_attention(const View &v, const Batch &b, uint32_t n_heads, const Rows
     a.window = window;
     a.sign = std::signbit(scale) ? -1.f : 1.f;
     a.scale2 = fabsf(scale) * 1.44269504f;
-    const Kind kind = kind_of(v, b.n_rows, b.starts || !b.lens, a.n_rep);
+    const Kind kind = kind_of(v, b.n_rows, b.starts || !b.lens, a.n_rep, n_cu);
     while ((1ull << a.rep_shift) < a.n_rep) a.rep_shift++;
     a.rep_mul = (uint32_t)((((1ull << a.rep_shift) - a.n_rep) << 32) / a.n_rep + 1);
     // a block for each wave of few_k, two of many_k; more where the chunks
     // would not be counted in 31 bits (all tiles seeing the whole cache)
     a.chunk = kind == kFew ? 4u : 2u;
-    a.lead = kind == kFew ? 0u : 4u;
+    // measured (cycles): an item costs few_k 30000 and many_k 20000 whatever its
+    // length, a chunk 5500 and 4800; items of one length each need no balance
+    a.lead = kind == kFew && v.n_seqs == 1 ? 0u : 4u;
     const uint64_t tiles = ((uint64_t)b.n_rows * a.n_rep + tile_rows(kind) - 1) / tile_rows(kind) + v.n_seqs;
     while (tiles * v.n_heads * (v.n_blocks / a.chunk + 1 + a.lead) >> 31) a.chunk *= 2;
     a.w = work_at(work, workgroups(n_cu), tile_rows(kind));
