@@ -383,34 +383,57 @@ class GpuContext:
         the most likely tokens [rows, k] of every row; torch device tensors
         (qg_logprobs_dev).  work: at least logprobs_work bytes."""
         rows, cols = logits.shape
-        if logits.stride(1) != 1 and cols > 1:
+        ld, step = logits.stride()
+        if step != 1 and cols > 1:
             raise QgemvError(7, "logits of a row are not contiguous")
         given = tokens.shape[1] if tokens is not None else 0
         k = top_ids.shape[1] if top_ids is not None else 0
-        for t, size, n in ((tokens, 4, rows * given), (logprobs, 4, rows * given), (entropy, 4, rows),
-                           (top_ids, 4, rows * k), (top_logprobs, 4, rows * k)):
-            if t is not None and (t.element_size() != size or t.numel() != n or not t.is_contiguous()):
-                raise QgemvError(7, "an array of logprobs_dev has another shape or type, or is not contiguous")
-        self.check(self.lib.qg_logprobs_dev(self.h, _ptr(logits), _row_type(logits), rows, cols, logits.stride(0),
-                                            _ptr(tokens), given, _ptr(logprobs), _ptr(entropy), k, _ptr(top_ids),
-                                            _ptr(top_logprobs), _ptr(work), _nbytes(work),
-                                            ctypes.c_void_p(stream) if stream else None), "qg_logprobs_dev")
+        rc = self.lib.qg_logprobs_dev(self.h, logits.data_ptr(), _row_type(logits), rows, cols, ld,
+                                      _words(tokens, rows * given, "tokens"), given, _words(logprobs, rows * given, "logprobs"),
+                                      _words(entropy, rows, "entropy"), k, _words(top_ids, rows * k, "top_ids"),
+                                      _words(top_logprobs, rows * k, "top_logprobs"), _addr(work), _nbytes(work), stream or None)
+        if rc:
+            self.check(rc, "qg_logprobs_dev")
+
+
+# The calls of include/qgops.h come once per layer and token, so their wrappers
+# keep to what a call needs (addresses as plain integers, one look at a tensor's
+# shape and strides).
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _nbytes(t) -> int:
     return 0 if t is None else t.numel() * t.element_size()
 
 
+_row_types: dict = {}
+
+
 def _row_type(t) -> int:
     """GGML id of a torch tensor's type (any but float32 and float16: one the library refuses)."""
-    return {"torch.float32": F32, "torch.float16": F16}.get(str(t.dtype), 0xFFFFFFFF)
+    if not _row_types:
+        import torch
+        _row_types.update({torch.float32: F32, torch.float16: F16})
+    return _row_types.get(t.dtype, 0xFFFFFFFF)
+
+
+def _words(t, n: int, what: str):
+    """Address of n contiguous 4-byte values."""
+    if t is None:
+        return None
+    if t.numel() != n or t.dtype.itemsize != 4 or not t.is_contiguous():
+        raise QgemvError(7, f"{what}: {n} contiguous values of 4 bytes")
+    return t.data_ptr()
 
 
 def _rows(t, n_rows: int, heads: int, hd: int, what: str) -> Rows:
     """qg_rows of a torch tensor [rows, heads, head_dim]."""
-    if tuple(t.shape) != (n_rows, heads, hd) or (hd > 1 and t.stride(2) != 1):
+    s = t.stride()
+    if t.shape != (n_rows, heads, hd) or (s[2] != 1 and hd > 1):
         raise QgemvError(7, f"{what} is not [{n_rows}, {heads}, {hd}] with contiguous elements")
-    return Rows(t.data_ptr(), _row_type(t), t.stride(0), t.stride(1))
+    return Rows(t.data_ptr(), _row_type(t), s[0], s[1])
 
 
 class Kv8Cache:
@@ -440,30 +463,27 @@ class Kv8Cache:
         return n.value
 
     def _batch(self, n_rows: int, lens, starts) -> Batch:
-        for t, n in ((lens, self.n_seqs), (starts, self.n_seqs + 1)):
-            if t is not None and (t.element_size() != 4 or t.numel() != n or not t.is_contiguous()):
-                raise QgemvError(7, "lens or starts: one int32 per sequence, one more of the starts")
-        return Batch(n_rows, _ptr(starts), _ptr(lens))
+        return Batch(n_rows, _words(starts, self.n_seqs + 1, "starts"), _words(lens, self.n_seqs, "lens"))
 
     def write_dev(self, k, v, lens, starts=None, stream=None):
         """Cache k and v [rows, n_kv_heads, head_dim]; lens: every sequence's
         positions with these rows (qg_kv8_write_dev)."""
-        n = k.shape[0]
-        b = self._batch(n, lens, starts)
-        rk, rv = (_rows(t, n, self.n_kv_heads, self.head_dim, w) for t, w in ((k, "k"), (v, "v")))
-        self.ctx.check(self.ctx.lib.qg_kv8_write_dev(self.ctx.h, self.h, ctypes.byref(b), ctypes.byref(rk),
-                                                     ctypes.byref(rv), ctypes.c_void_p(stream) if stream else None),
-                       "qg_kv8_write_dev")
+        n, heads, hd = k.shape[0], self.n_kv_heads, self.head_dim
+        rc = self.ctx.lib.qg_kv8_write_dev(self.ctx.h, self.h, ctypes.byref(self._batch(n, lens, starts)),
+                                           ctypes.byref(_rows(k, n, heads, hd, "k")),
+                                           ctypes.byref(_rows(v, n, heads, hd, "v")), stream or None)
+        if rc:
+            self.ctx.check(rc, "qg_kv8_write_dev")
 
     def read_dev(self, seq: int, n_seqs: int, pos: int, n: int, k=None, v=None, stream=None):
         """Positions pos .. pos + n of n_seqs sequences from seq on as values
         [n_seqs * n, n_kv_heads, head_dim] (qg_kv8_read_dev)."""
-        rk, rv = (None if t is None else _rows(t, n_seqs * n, self.n_kv_heads, self.head_dim, w)
-                  for t, w in ((k, "k"), (v, "v")))
-        self.ctx.check(self.ctx.lib.qg_kv8_read_dev(self.ctx.h, self.h, seq, n_seqs, pos, n,
-                                                    None if rk is None else ctypes.byref(rk),
-                                                    None if rv is None else ctypes.byref(rv),
-                                                    ctypes.c_void_p(stream) if stream else None), "qg_kv8_read_dev")
+        r, heads, hd = n_seqs * n, self.n_kv_heads, self.head_dim
+        rc = self.ctx.lib.qg_kv8_read_dev(self.ctx.h, self.h, seq, n_seqs, pos, n,
+                                          None if k is None else ctypes.byref(_rows(k, r, heads, hd, "k")),
+                                          None if v is None else ctypes.byref(_rows(v, r, heads, hd, "v")), stream or None)
+        if rc:
+            self.ctx.check(rc, "qg_kv8_read_dev")
 
     def attention_work(self, n_rows: int, n_heads: int) -> int:
         """Bytes of workspace attention_dev needs (qg_kv8_attention_work)."""
@@ -475,13 +495,13 @@ class Kv8Cache:
     def attention_dev(self, q, out, lens, work=None, starts=None, scale=None, window: int = 0, stream=None):
         """out = attention of q [rows, n_heads, head_dim] over the cache; scale:
         1 / sqrt(head_dim) by default (qg_kv8_attention_dev)."""
-        n, heads = q.shape[0], q.shape[1]
-        b = self._batch(n, lens, starts)
-        rq, ro = (_rows(t, n, heads, self.head_dim, w) for t, w in ((q, "q"), (out, "out")))
-        self.ctx.check(self.ctx.lib.qg_kv8_attention_dev(
-            self.ctx.h, self.h, ctypes.byref(b), heads, ctypes.byref(rq),
-            float(self.head_dim ** -0.5 if scale is None else scale), window, ctypes.byref(ro), _ptr(work), _nbytes(work),
-            ctypes.c_void_p(stream) if stream else None), "qg_kv8_attention_dev")
+        n, heads, hd = q.shape[0], q.shape[1], self.head_dim
+        rc = self.ctx.lib.qg_kv8_attention_dev(
+            self.ctx.h, self.h, ctypes.byref(self._batch(n, lens, starts)), heads, ctypes.byref(_rows(q, n, heads, hd, "q")),
+            hd ** -0.5 if scale is None else scale, window, ctypes.byref(_rows(out, n, heads, hd, "out")), _addr(work),
+            _nbytes(work), stream or None)
+        if rc:
+            self.ctx.check(rc, "qg_kv8_attention_dev")
 
 
 class DeviceMatrix:

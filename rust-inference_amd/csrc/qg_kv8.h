@@ -127,7 +127,7 @@ __device__ __forceinline__ void store1(const Rows &r, uint64_t at, float v)
 }
 
 // Launchers; 0, or -1 for a failed launch (hipGetLastError holds it).
-int launch_write(const View &c, const Batch &b, const Rows &k, const Rows &v, hipStream_t st);
+int launch_write(const View &c, const Batch &b, const Rows &k, const Rows &v, int n_cu, hipStream_t st);
 int launch_read(const View &c, uint32_t seq, uint32_t n_seqs, uint32_t pos, uint32_t n, const Rows *k, const Rows *v,
                 hipStream_t st);
 int launch_attention(const View &c, const Batch &b, uint32_t n_heads, const Rows &q, float scale, uint32_t window,

@@ -38,22 +38,29 @@ __device__ __forceinline__ Piece piece_of(const Batch &b, uint32_t seq, uint32_t
     return p;
 }
 
-// The sequence and item of workgroup `want`: the items of the sequences before
-// it are counted 64 sequences at a time, by every wave on its own.  False
-// behind the last item.
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, uint32_t l)
+{
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)l);
+}
+
+// The sequence, its piece and the item of workgroup `want`: the items of the
+// sequences before it are counted 64 sequences at a time, by every wave on its
+// own.  False behind the last item.
 __device__ bool find_item(const Batch &b, uint32_t n_seqs, uint32_t max_len, uint32_t want, uint32_t *seq,
-                          uint32_t *item)
+                          uint32_t *item, Piece *piece)
 {
     const uint32_t lane = threadIdx.x & 63u;
     if (b.lens && !b.starts) {                       // one row each
         *seq = want;
         *item = 0;
-        return piece_of(b, want, max_len).items != 0;
+        *piece = piece_of(b, want, max_len);
+        return piece->items != 0;
     }
     uint32_t before = 0;
     for (uint32_t s0 = 0; s0 < n_seqs; s0 += 64) {
-        uint32_t n = s0 + lane < n_seqs ? piece_of(b, s0 + lane, max_len).items : 0u;
-        const uint32_t own = n;
+        Piece p{};
+        if (s0 + lane < n_seqs) p = piece_of(b, s0 + lane, max_len);
+        uint32_t n = p.items;
 #pragma unroll
         for (uint32_t o = 1; o < 64; o <<= 1) {
             const uint32_t up = (uint32_t)__shfl_up((int)n, o, 64);
@@ -61,12 +68,21 @@ __device__ bool find_item(const Batch &b, uint32_t n_seqs, uint32_t max_len, uin
         }
         const uint64_t past = __ballot(before + n > want);
         if (past) {
-            const int l = __ffsll((unsigned long long)past) - 1;
-            *seq = s0 + (uint32_t)l;
-            *item = want - (before + (uint32_t)__shfl((int)(n - own), l, 64));
+            const uint32_t l = (uint32_t)__ffsll((unsigned long long)past) - 1;
+            *seq = s0 + l;
+            *item = want - (before + lane_of(n - p.items, l));
+            piece->s.row = lane_of(p.s.row, l);
+            piece->s.n = lane_of(p.s.n, l);
+            piece->s.len = lane_of(p.s.len, l);
+            piece->s.pos = (int64_t)piece->s.len - (int64_t)piece->s.n;
+            piece->first = lane_of(p.first, l);
+            piece->end = lane_of(p.end, l);
+            piece->b0 = lane_of(p.b0, l);
+            piece->bl = lane_of(p.bl, l);
+            piece->items = lane_of(p.items, l);
             return true;
         }
-        before += (uint32_t)__shfl((int)n, 63, 64);
+        before += lane_of(n, 63);
     }
     return false;
 }
@@ -102,7 +118,7 @@ __device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint6
     uint32_t *tail_max = v.tail_max + (base * 2 + (uint32_t)(slot < 0 ? 0 : slot)) * kBlock;
     float val[NC][16];
     const bool fresh = t >= lo && t < hi, old = t < lo;
-    const float s_old = *scale;
+    const float s_old = lo ? *scale : 0.f;
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < NC; i++) {
@@ -196,22 +212,24 @@ __device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint6
     __syncthreads();
 }
 
-// Grid: (items, heads, keys / values).
+// Grid: (items, heads, keys / values).  Bound by the latency of a few dependent
+// loads; WAVES: workgroups of which a compute unit holds at least so many (fewer
+// registers for each).
 //
 // The scale of a block follows from its largest magnitude, so a new token in a
 // block that is partly there costs its own row and 32 remembered magnitudes
 // while it is not the largest, and the block's f32 rows (kept in one of two
 // slots) when it is.  Two slots, because a call that ends one block and opens
 // another must leave the values of the first: the same call may come again.
-template <int NC> __global__ void __launch_bounds__(256) write_k(View v, Batch b, Rows k, Rows val)
+template <int NC, int WAVES> __global__ void __launch_bounds__(256, WAVES) write_k(View v, Batch b, Rows k, Rows val)
 {
     __shared__ uint32_t maxes[kBlock], red[4];
     __shared__ __attribute__((aligned(16))) uint8_t stage[kBlock * (128 * NC + 16)];
     uint32_t seq, item;
-    if (!find_item(b, v.n_seqs, v.max_len, blockIdx.x, &seq, &item)) return;
+    Piece p;
+    if (!find_item(b, v.n_seqs, v.max_len, blockIdx.x, &seq, &item, &p)) return;
     const bool key = blockIdx.z == 0;
     const Rows &x = key ? k : val;
-    const Piece p = piece_of(b, seq, v.max_len);
     const uint32_t head = blockIdx.y, sh = seq * v.n_heads + head;
     const uint64_t base = (uint64_t)blockIdx.z * v.n_seqs * v.n_heads + sh;
     // element of the row that holds position pos
@@ -320,15 +338,20 @@ int launched()
 
 }  // namespace
 
-int launch_write(const View &v, const Batch &b, const Rows &k, const Rows &x, hipStream_t st)
+int launch_write(const View &v, const Batch &b, const Rows &k, const Rows &x, int n_cu, hipStream_t st)
 {
     if (b.n_rows == 0) return 0;
     // items of a sequence of n rows: at most (n + 30) / 32 + 1, and one for one row
     const uint64_t most = b.starts ? (uint64_t)b.n_rows / kBlock + 2ull * std::min(v.n_seqs, b.n_rows)
                           : b.lens ? b.n_rows : b.n_rows / kBlock + 2u;
     const dim3 grid((uint32_t)most, v.n_heads, 2);
-    if (v.dp <= 128) hipLaunchKernelGGL(write_k<1>, grid, dim3(256), 0, st, v, b, k, x);
-    else hipLaunchKernelGGL(write_k<2>, grid, dim3(256), 0, st, v, b, k, x);
+    // more workgroups than fit with the registers they would like (5 a compute
+    // unit): as many as there can be (us: 32 prompts of up to 2048 tokens 62.4
+    // against 73.1; 1001 tokens 9.1 against 8.5, one token 5.2 against 4.6)
+    const bool crowd = most * v.n_heads * 2 > 5ull * (uint32_t)(n_cu > 0 ? n_cu : 256);
+    if (v.dp > 128) hipLaunchKernelGGL((write_k<2, 1>), grid, dim3(256), 0, st, v, b, k, x);
+    else if (crowd) hipLaunchKernelGGL((write_k<1, 8>), grid, dim3(256), 0, st, v, b, k, x);
+    else hipLaunchKernelGGL((write_k<1, 1>), grid, dim3(256), 0, st, v, b, k, x);
     return launched();
 }
 
@@ -535,7 +558,7 @@ int qg_kv8_write_dev(qg_ctx *ctx, qg_kv8 *kv, const qg_batch *batch, const qg_ro
     if (b.n_rows == 0) return QG_OK;
     const hipError_t e = hipSetDevice(ctx->device);
     if (e != hipSuccess) return qg_fail(ctx, QG_ERR_HIP, "hipSetDevice", e);
-    return launch_status(ctx, qg8::launch_write(kv->v, b, rk, rv, pick(ctx, stream)), "cache write");
+    return launch_status(ctx, qg8::launch_write(kv->v, b, rk, rv, ctx->n_cu, pick(ctx, stream)), "cache write");
 }
 
 int qg_kv8_read_dev(qg_ctx *ctx, const qg_kv8 *kv, size_t seq, size_t n_seqs, size_t pos, size_t n, const qg_rows *k,

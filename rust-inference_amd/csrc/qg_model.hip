@@ -1384,7 +1384,7 @@ int kv8_attention(qg_model *m, uint32_t l, const qg8::Batch &b, const float *q, 
                   const float *v, size_t ldv, float *out)
 {
     const qg8::View &c = m->kv8[l]->v;
-    if (qg8::launch_write(c, b, kv8_rows(m, k, ldk), kv8_rows(m, v, ldv), m->ctx->stream) ||
+    if (qg8::launch_write(c, b, kv8_rows(m, k, ldk), kv8_rows(m, v, ldv), m->ctx->n_cu, m->ctx->stream) ||
         qg8::launch_attention(c, b, m->cfg.n_heads, kv8_rows(m, q, ldq), 1.0f / sqrtf((float)m->hd), 0,
                               kv8_rows(m, out, m->q_dim), m->kv8_work, m->ctx->n_cu, m->ctx->stream))
         return mfail(m, QG_ERR_HIP, "attention over the 8-bit cache", hipGetLastError());
