@@ -60,14 +60,14 @@ __device__ __forceinline__ Sums join(Sums a, Sums b)
 // Over the workgroup, to all threads.
 __device__ Sums join_all(Sums a, Sums *red)
 {
-#pragma unroll
+#pragma unroll 1
     for (int o = 32; o > 0; o >>= 1)
         a = join(a, Sums{__shfl_xor(a.m, o, 64), __shfl_xor(a.z, o, 64), __shfl_xor(a.s, o, 64)});
     __syncthreads();
     if ((threadIdx.x & 63u) == 0) red[threadIdx.x >> 6] = a;
     __syncthreads();
     a = red[0];
-#pragma unroll
+#pragma unroll 1
     for (uint32_t i = 1; i < kThreads / 64; i++) a = join(a, red[i]);
     return a;
 }
@@ -85,12 +85,29 @@ __device__ __forceinline__ float value_of(uint64_t key)
     return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
 }
 
-// LDS of the selection: candidates, the threads' largest keys, the best so far,
-// floor_of's answer, the number of candidates.
+// LDS of the selection: the threads' largest keys, candidates and what is left of
+// them, the best so far, floor_of's answer, the number of candidates.
 template <uint32_t CAP> struct Pick {
-    uint64_t cand[CAP], top[kThreads], best[kMaxK], floor;
+    static constexpr uint32_t kRounds = (CAP + kThreads - 1) / kThreads;
+    uint64_t top[kThreads], cand[CAP], left[CAP > kThreads ? kMaxK * kRounds : 1], best[kMaxK], floor;
     uint32_t n;
 };
+
+// How many of n keys (16-byte aligned, zeros up to a multiple of 16) are larger:
+// sixteen at a time, their reads one behind the other.
+__device__ __forceinline__ uint32_t count_larger(const uint64_t *keys, uint32_t n, uint64_t key)
+{
+    uint32_t c = 0;
+#pragma unroll 2
+    for (uint32_t i = 0; i < n; i += 16) {
+        ulonglong2 t[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++) t[j] = *(const ulonglong2 *)&keys[i + 2 * j];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++) c += (t[j].x > key ? 1u : 0u) + (t[j].y > key ? 1u : 0u);
+    }
+    return c;
+}
 
 // The k-th largest of the threads' keys (0: fewer than k have one).
 template <uint32_t CAP> __device__ uint64_t floor_of(Pick<CAP> &p, uint64_t key, uint32_t k)
@@ -99,11 +116,7 @@ template <uint32_t CAP> __device__ uint64_t floor_of(Pick<CAP> &p, uint64_t key,
     p.top[threadIdx.x] = key;
     if (threadIdx.x == 0) p.floor = 0;
     __syncthreads();
-    uint32_t larger = 0;
-    for (uint32_t i = 0; i < kThreads; i += 2) {
-        const ulonglong2 t = *(const ulonglong2 *)&p.top[i];
-        larger += (t.x > key ? 1u : 0u) + (t.y > key ? 1u : 0u);
-    }
+    const uint32_t larger = count_larger(p.top, kThreads, key);
     if (key && larger == k - 1) p.floor = key;               // one thread, or none
     __syncthreads();
     return p.floor;
@@ -112,32 +125,31 @@ template <uint32_t CAP> __device__ uint64_t floor_of(Pick<CAP> &p, uint64_t key,
 // The k largest of p.cand[0 .. p.n), in order, into p.best (0 behind them).
 template <uint32_t CAP> __device__ void rank(Pick<CAP> &p, uint32_t k)
 {
-    constexpr uint32_t R = (CAP + kThreads - 1) / kThreads;
+    uint64_t *from = p.cand, *to = p.left;
     __syncthreads();
-    while (p.n > kThreads) {                                  // at most k R are left each time
-        uint64_t own[R], top = 0;
-        const uint32_t n = p.n;
-#pragma unroll
-        for (uint32_t i = 0; i < R; i++) {
-            const uint32_t at = threadIdx.x + i * kThreads;
-            own[i] = at < n ? p.cand[at] : 0ull;
-            top = own[i] > top ? own[i] : top;
-        }
+    uint32_t n = p.n;
+    while (n > kThreads) {                    // at most k ceil(n / 256) are left each time
+        uint64_t top = 0;
+#pragma unroll 1
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) top = from[i] > top ? from[i] : top;
         const uint64_t f = floor_of(p, top, k);
         if (threadIdx.x == 0) p.n = 0;
         __syncthreads();
-#pragma unroll
-        for (uint32_t i = 0; i < R; i++)
-            if (own[i] && own[i] >= f) p.cand[atomicAdd(&p.n, 1u)] = own[i];
+        if (top && top >= f)
+#pragma unroll 1
+            for (uint32_t i = threadIdx.x; i < n; i += kThreads)
+                if (from[i] && from[i] >= f) to[atomicAdd(&p.n, 1u)] = from[i];
         __syncthreads();
+        n = p.n;
+        uint64_t *const t = from;
+        from = to;
+        to = t;
     }
-    const uint32_t n = p.n;
-    const uint64_t own = threadIdx.x < n ? p.cand[threadIdx.x] : 0ull;
-    uint32_t larger = 0;
-    for (uint32_t i = 0; i < n; i++) larger += p.cand[i] > own ? 1u : 0u;
-    __syncthreads();
+    const uint64_t own = threadIdx.x < n ? from[threadIdx.x] : 0ull;
+    p.top[threadIdx.x] = own;
     if (threadIdx.x < k) p.best[threadIdx.x] = 0;
     __syncthreads();
+    const uint32_t larger = count_larger(p.top, n, own);
     if (own && larger < k) p.best[larger] = own;
     __syncthreads();
 }
@@ -214,33 +226,29 @@ template <int E, bool F16, bool TOP> __global__ void __launch_bounds__(kThreads)
             }
         all = join(all, t);
         if (TOP) {
+            // element n of the thread (vector n / VE)
             const int64_t own0 = c + (int64_t)threadIdx.x * VE;
-            auto inside = [&](uint32_t i, uint32_t j, uint32_t *id) {
-                const int64_t k = own0 + (int64_t)i * kThreads * VE + j;
-                *id = (uint32_t)k;
-                return k >= (int64_t)lo && k < (int64_t)hi;
+            auto id_of = [&](uint32_t n) { return own0 + (int64_t)(n / VE) * (kThreads * VE) + n % VE; };
+            // its key, read once more (0 outside of the part)
+            auto key_at = [&](uint32_t n) {
+                const int64_t k = id_of(n);
+                if (k < (int64_t)lo || k >= (int64_t)hi) return 0ull;
+                return (unsigned long long)key_of(F16 ? (float)((const _Float16 *)x)[k] : ((const float *)x)[k], (uint32_t)k);
             };
             // the thread's largest key: the first of its largest values (t.m is
-            // kLowest at least: such rows look at every element)
+            // kLowest at least: where it is, every element is looked at)
             uint64_t top = 0;
             if (t.m > kLowest) {
+                uint32_t n = 0;
 #pragma unroll
-                for (int i = NV - 1; i >= 0; i--)
-#pragma unroll
-                    for (int j = VE - 1; j >= 0; j--) {
-                        uint32_t id;
-                        (void)inside(i, j, &id);
-                        if (v[i][j] == t.m) top = key_of(t.m, id);
-                    }
+                for (int i = E - 1; i >= 0; i--) n = v[i / VE][i % VE] == t.m ? (uint32_t)i : n;
+                top = key_of(t.m, (uint32_t)id_of(n));
             } else {
-#pragma unroll
-                for (uint32_t i = 0; i < NV; i++)
-#pragma unroll
-                    for (uint32_t j = 0; j < VE; j++) {
-                        uint32_t id;
-                        const uint64_t key = inside(i, j, &id) ? key_of(v[i][j], id) : 0ull;
-                        top = key > top ? key : top;
-                    }
+#pragma unroll 1
+                for (uint32_t n = 0; n < E; n++) {
+                    const uint64_t key = key_at(n);
+                    top = key > top ? key : top;
+                }
             }
             if (__syncthreads_or(top > least)) {
                 const uint64_t f = floor_of(pick, top, a.k);
@@ -249,15 +257,19 @@ template <int E, bool F16, bool TOP> __global__ void __launch_bounds__(kThreads)
                 __syncthreads();
                 if (threadIdx.x < a.k && pick.best[threadIdx.x])
                     pick.cand[atomicAdd(&pick.n, 1u)] = pick.best[threadIdx.x];
-                if (top >= from)
+                if (top >= from) {
+                    // the elements that are as large as the floor's value by their
+                    // bits, then their keys
+                    const float y = from >> 32 ? value_of(from) : -INFINITY;
+                    uint64_t some = 0;
 #pragma unroll
-                    for (uint32_t i = 0; i < NV; i++)
-#pragma unroll
-                        for (uint32_t j = 0; j < VE; j++) {
-                            uint32_t id;
-                            const uint64_t key = inside(i, j, &id) ? key_of(v[i][j], id) : 0ull;
-                            if (key >= from) pick.cand[atomicAdd(&pick.n, 1u)] = key;
-                        }
+                    for (int i = 0; i < E; i++) some |= v[i / VE][i % VE] >= y ? 1ull << i : 0ull;
+#pragma unroll 1
+                    for (; some; some &= some - 1) {
+                        const uint64_t key = key_at((uint32_t)__ffsll((unsigned long long)some) - 1);
+                        if (key >= from) pick.cand[atomicAdd(&pick.n, 1u)] = key;
+                    }
+                }
                 rank(pick, a.k);
                 least = pick.best[a.k - 1];
             }
@@ -286,12 +298,10 @@ template <bool F16, bool TOP> __global__ void __launch_bounds__(kThreads) final_
         t = Sums{w.x, w.y, w.z};
     }
     if (TOP) {
-        if (threadIdx.x == 0) pick.n = 0;
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < a.parts * a.k; i += kThreads) {
-            const uint64_t key = a.keys[row * a.parts * a.k + i];
-            if (key) pick.cand[atomicAdd(&pick.n, 1u)] = key;
-        }
+        if (threadIdx.x == 0) pick.n = a.parts * a.k;
+#pragma unroll 8
+        for (uint32_t i = threadIdx.x; i < a.parts * a.k; i += kThreads)
+            pick.cand[i] = a.keys[row * a.parts * a.k + i];
         rank(pick, a.k);
     }
     t = join_all(t, red);
