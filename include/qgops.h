@@ -48,6 +48,7 @@ typedef struct qg_rows {
  * stand.  Sequence s has the rows d_starts[s] .. d_starts[s + 1) (n_seqs + 1
  * values, not decreasing, the last one at most n_rows), or, with d_starts
  * NULL, the single row s (n_rows must then be n_seqs, else QG_ERR_SHAPE).
+ * n_rows is below 2^28 (QG_ERR_SHAPE).
  * d_lens[s] counts its positions with this call's tokens included: row i of
  * its n rows stands at position d_lens[s] - n + i.  A sequence without rows
  * takes no part; rows behind the last sequence's are neither read nor
@@ -72,8 +73,8 @@ typedef struct qg_batch {
 typedef struct qg_kv8 qg_kv8;
 enum { QG_KV8_BLOCK = 32 };
 
-/* n_seqs, n_kv_heads 1 .. 65535, head_dim 1 .. 256, max_len 1 .. 2^31 - 32
- * (QG_ERR_SHAPE otherwise).  An empty cache, all zero; synchronous. */
+/* n_seqs, n_kv_heads 1 .. 65535 and 2^26 at most together, head_dim 1 .. 256,
+ * max_len 1 .. 2^31 - 32 (QG_ERR_SHAPE otherwise).  An empty cache, all zero; synchronous. */
 int qg_kv8_create(qg_ctx *ctx, size_t n_seqs, size_t n_kv_heads, size_t head_dim, size_t max_len, qg_kv8 **out);
 /* QG_ERR_INVALID_ARG for a handle this context does not hold.  The caller has
  * waited for its own streams; qg_destroy frees what is left. */
@@ -93,7 +94,8 @@ int qg_kv8_write_dev(qg_ctx *ctx, qg_kv8 *kv, const qg_batch *batch, const qg_ro
 
 /* Positions pos .. pos + n of sequences seq .. seq + n_seqs as values: row
  * (i * n + j) of k and v is position pos + j of sequence seq + i.  Either
- * output may be NULL.  QG_ERR_SHAPE outside the cache.  Positions behind a
+ * output may be NULL.  QG_ERR_SHAPE outside the cache, for n of 2^28 or more, and
+ * for keys and values of more than 65535 heads together.  Positions behind a
  * sequence's last read as zero in a new cache, else as what is left there. */
 int qg_kv8_read_dev(qg_ctx *ctx, const qg_kv8 *kv, size_t seq, size_t n_seqs, size_t pos, size_t n, const qg_rows *k,
                     const qg_rows *v, void *stream);
@@ -104,10 +106,11 @@ int qg_kv8_read_dev(qg_ctx *ctx, const qg_kv8 *kv, size_t seq, size_t n_seqs, si
  *   out = sum_j p_j v_j,  p = softmax over j of scale * q . k_j,
  * for the row at position p over the positions j <= p, and j > p - window
  * where window is not 0.  Rows see the values as they are after the call's
- * writes: a later token of the same block may have moved its scale.  A row with no position to see (one below 0) gives
- * zeros; a row at a position past max_len sees the positions there are.  q and
- * out have one type; f32 rows are computed to f32 precision (two f16 pieces of
- * q and of p), f16 rows with f16 p, sums in f32.  d_work: qg_kv8_attention_work
+ * writes: a later token of the same block may have moved its scale.  A row with
+ * no position to see (one below 0) gives zeros; a row at a position past max_len
+ * sees the positions there are.  n_heads at most 65535, n_rows * n_heads below
+ * 2^31 (QG_ERR_SHAPE).  q and out have one type; f32 rows are computed to f32
+ * precision (two f16 pieces of q and of p), f16 rows with f16 p, sums in f32.  d_work: qg_kv8_attention_work
  * bytes of device memory (16-byte aligned) that no other call in flight uses
  * (captured graphs that may run side by side need one each); its contents need
  * not be kept.  QG_ERR_SHAPE when work_bytes is less. */
@@ -129,7 +132,8 @@ int qg_kv8_attention_work(qg_ctx *ctx, const qg_kv8 *kv, size_t n_rows, size_t n
  * -inf.  In a row that holds a NaN or +inf, or -inf only, every probability and
  * the entropy are NaN (the ids still are the largest logits).  Sums in f32.
  * d_work: qg_logprobs_work bytes (16-byte aligned), as for
- * qg_kv8_attention_dev.  n_cols 1 .. 2^31 - 1. */
+ * qg_kv8_attention_dev.  n_rows below 2^24, n_cols 1 .. 2^31 - 1, rows ld >=
+ * n_cols apart (QG_ERR_SHAPE otherwise). */
 enum { QG_LOGPROBS_MAX_TOP = 64 };
 #define QG_TOKEN_NONE 0xFFFFFFFFu
 int qg_logprobs_dev(qg_ctx *ctx, const void *d_logits, uint32_t type, size_t n_rows, size_t n_cols, size_t ld,

@@ -266,6 +266,7 @@ class GpuContext:
         if rc != QG_OK:
             raise QgemvError(rc, f"qg_init(device={device})")
         self.h = h
+        self.device = device
         self._mats = []
 
     @classmethod
@@ -388,10 +389,13 @@ class GpuContext:
             raise QgemvError(7, "logits of a row are not contiguous")
         given = tokens.shape[1] if tokens is not None else 0
         k = top_ids.shape[1] if top_ids is not None else 0
-        rc = self.lib.qg_logprobs_dev(self.h, logits.data_ptr(), _row_type(logits), rows, cols, ld,
-                                      _words(tokens, rows * given, "tokens"), given, _words(logprobs, rows * given, "logprobs"),
-                                      _words(entropy, rows, "entropy"), k, _words(top_ids, rows * k, "top_ids"),
-                                      _words(top_logprobs, rows * k, "top_logprobs"), _addr(work), _nbytes(work), stream or None)
+        dev = self.device
+        rc = self.lib.qg_logprobs_dev(self.h, _addr(logits, dev, "logits"), _row_type(logits), rows, cols, ld,
+                                      _words(tokens, rows * given, dev, "tokens"), given,
+                                      _words(logprobs, rows * given, dev, "logprobs"), _words(entropy, rows, dev, "entropy"),
+                                      k, _words(top_ids, rows * k, dev, "top_ids"),
+                                      _words(top_logprobs, rows * k, dev, "top_logprobs"), _addr(work, dev, "work"),
+                                      _nbytes(work), stream or None)
         if rc:
             self.check(rc, "qg_logprobs_dev")
 
@@ -400,8 +404,13 @@ class GpuContext:
 # keep to what a call needs (addresses as plain integers, one look at a tensor's
 # shape and strides).
 
-def _addr(t):
-    return None if t is None else t.data_ptr()
+def _addr(t, dev: int, what: str):
+    """Address of a tensor on the context's device; None stays None."""
+    if t is None:
+        return None
+    if t.get_device() != dev:
+        raise QgemvError(1, f"{what}: a tensor on the context's device")
+    return t.data_ptr()
 
 
 def _nbytes(t) -> int:
@@ -419,21 +428,21 @@ def _row_type(t) -> int:
     return _row_types.get(t.dtype, 0xFFFFFFFF)
 
 
-def _words(t, n: int, what: str):
+def _words(t, n: int, dev: int, what: str):
     """Address of n contiguous 4-byte values."""
     if t is None:
         return None
     if t.numel() != n or t.dtype.itemsize != 4 or not t.is_contiguous():
         raise QgemvError(7, f"{what}: {n} contiguous values of 4 bytes")
-    return t.data_ptr()
+    return _addr(t, dev, what)
 
 
-def _rows(t, n_rows: int, heads: int, hd: int, what: str) -> Rows:
+def _rows(t, n_rows: int, heads: int, hd: int, dev: int, what: str) -> Rows:
     """qg_rows of a torch tensor [rows, heads, head_dim]."""
     s = t.stride()
     if t.shape != (n_rows, heads, hd) or (s[2] != 1 and hd > 1):
         raise QgemvError(7, f"{what} is not [{n_rows}, {heads}, {hd}] with contiguous elements")
-    return Rows(t.data_ptr(), _row_type(t), s[0], s[1])
+    return Rows(_addr(t, dev, what), _row_type(t), s[0], s[1])
 
 
 class Kv8Cache:
@@ -463,25 +472,26 @@ class Kv8Cache:
         return n.value
 
     def _batch(self, n_rows: int, lens, starts) -> Batch:
-        return Batch(n_rows, _words(starts, self.n_seqs + 1, "starts"), _words(lens, self.n_seqs, "lens"))
+        dev = self.ctx.device
+        return Batch(n_rows, _words(starts, self.n_seqs + 1, dev, "starts"), _words(lens, self.n_seqs, dev, "lens"))
 
     def write_dev(self, k, v, lens, starts=None, stream=None):
         """Cache k and v [rows, n_kv_heads, head_dim]; lens: every sequence's
         positions with these rows (qg_kv8_write_dev)."""
-        n, heads, hd = k.shape[0], self.n_kv_heads, self.head_dim
+        n, heads, hd, dev = k.shape[0], self.n_kv_heads, self.head_dim, self.ctx.device
         rc = self.ctx.lib.qg_kv8_write_dev(self.ctx.h, self.h, ctypes.byref(self._batch(n, lens, starts)),
-                                           ctypes.byref(_rows(k, n, heads, hd, "k")),
-                                           ctypes.byref(_rows(v, n, heads, hd, "v")), stream or None)
+                                           ctypes.byref(_rows(k, n, heads, hd, dev, "k")),
+                                           ctypes.byref(_rows(v, n, heads, hd, dev, "v")), stream or None)
         if rc:
             self.ctx.check(rc, "qg_kv8_write_dev")
 
     def read_dev(self, seq: int, n_seqs: int, pos: int, n: int, k=None, v=None, stream=None):
         """Positions pos .. pos + n of n_seqs sequences from seq on as values
         [n_seqs * n, n_kv_heads, head_dim] (qg_kv8_read_dev)."""
-        r, heads, hd = n_seqs * n, self.n_kv_heads, self.head_dim
+        r, heads, hd, dev = n_seqs * n, self.n_kv_heads, self.head_dim, self.ctx.device
         rc = self.ctx.lib.qg_kv8_read_dev(self.ctx.h, self.h, seq, n_seqs, pos, n,
-                                          None if k is None else ctypes.byref(_rows(k, r, heads, hd, "k")),
-                                          None if v is None else ctypes.byref(_rows(v, r, heads, hd, "v")), stream or None)
+                                          None if k is None else ctypes.byref(_rows(k, r, heads, hd, dev, "k")),
+                                          None if v is None else ctypes.byref(_rows(v, r, heads, hd, dev, "v")), stream or None)
         if rc:
             self.ctx.check(rc, "qg_kv8_read_dev")
 
@@ -495,11 +505,11 @@ class Kv8Cache:
     def attention_dev(self, q, out, lens, work=None, starts=None, scale=None, window: int = 0, stream=None):
         """out = attention of q [rows, n_heads, head_dim] over the cache; scale:
         1 / sqrt(head_dim) by default (qg_kv8_attention_dev)."""
-        n, heads, hd = q.shape[0], q.shape[1], self.head_dim
+        n, heads, hd, dev = q.shape[0], q.shape[1], self.head_dim, self.ctx.device
         rc = self.ctx.lib.qg_kv8_attention_dev(
-            self.ctx.h, self.h, ctypes.byref(self._batch(n, lens, starts)), heads, ctypes.byref(_rows(q, n, heads, hd, "q")),
-            hd ** -0.5 if scale is None else scale, window, ctypes.byref(_rows(out, n, heads, hd, "out")), _addr(work),
-            _nbytes(work), stream or None)
+            self.ctx.h, self.h, ctypes.byref(self._batch(n, lens, starts)), heads, ctypes.byref(_rows(q, n, heads, hd, dev, "q")),
+            hd ** -0.5 if scale is None else scale, window, ctypes.byref(_rows(out, n, heads, hd, dev, "out")),
+            _addr(work, dev, "work"), _nbytes(work), stream or None)
         if rc:
             self.ctx.check(rc, "qg_kv8_attention_dev")
 

@@ -379,7 +379,11 @@ int check_kv8(qg_ctx *ctx, const qg_kv8 *kv)
     return QG_OK;
 }
 
-// a * b + c in 62 bits
+// Rows of a call, positions of a read: a launch counts its threads in 32 bits,
+// and 256 of them take 32 positions (and two part blocks of every sequence).
+constexpr size_t kMostRows = (size_t)1 << 28;
+
+// a * b + c, below 2^58: addresses in bytes fit
 bool fits(size_t a, size_t b, size_t c, size_t *out)
 {
     size_t t;
@@ -419,7 +423,7 @@ int check_rows(qg_ctx *ctx, const qg_rows *r, size_t n, size_t heads, size_t hd,
 int check_batch(qg_ctx *ctx, const qg_kv8 *kv, const qg_batch *b, qg8::Batch *out)
 {
     if (!b) return qg_fail(ctx, QG_ERR_INVALID_ARG, "batch is NULL");
-    if (b->n_rows > 0x7FFFFFFFu) return qg_fail(ctx, QG_ERR_SHAPE, "too many rows");
+    if (b->n_rows >= kMostRows) return qg_fail(ctx, QG_ERR_SHAPE, "too many rows");
     if (!b->d_lens || ((uintptr_t)b->d_lens | (uintptr_t)b->d_starts) % 4)
         return qg_fail(ctx, QG_ERR_INVALID_ARG, "batch lengths missing or not aligned");
     if (!b->d_starts && b->n_rows != kv->v.n_seqs)
@@ -443,7 +447,7 @@ int launch_status(qg_ctx *ctx, int r, const char *what)
 int qg_kv8_make(qg_ctx *ctx, size_t n_seqs, size_t n_kv_heads, size_t head_dim, size_t max_len, qg_kv8 **out)
 {
     if (n_seqs < 1 || n_seqs > 65535 || n_kv_heads < 1 || n_kv_heads > 65535 || head_dim < 1 || head_dim > 256 ||
-        max_len < 1 || max_len > 0x7FFFFFE0u || n_seqs * n_kv_heads > 0x3FFFFFFFu)
+        max_len < 1 || max_len > 0x7FFFFFE0u || n_seqs * n_kv_heads > (size_t)1 << 26)
         return qg_fail(ctx, QG_ERR_SHAPE, "cache sizes");
     qg8::View v{};
     v.n_seqs = (uint32_t)n_seqs;
@@ -567,8 +571,9 @@ int qg_kv8_read_dev(qg_ctx *ctx, const qg_kv8 *kv, size_t seq, size_t n_seqs, si
     int rc = check_kv8(ctx, kv);
     if (rc) return rc;
     const qg8::View &c = kv->v;
-    if (seq > c.n_seqs || n_seqs > c.n_seqs - seq || pos > c.max_len || n > c.max_len - pos)
-        return qg_fail(ctx, QG_ERR_SHAPE, "positions outside the cache");
+    if (seq > c.n_seqs || n_seqs > c.n_seqs - seq || pos > c.max_len || n > c.max_len - pos ||
+        n >= kMostRows)
+        return qg_fail(ctx, QG_ERR_SHAPE, "positions outside the cache, or too many");
     qg8::Rows rk{}, rv{};
     if ((k && (rc = check_rows(ctx, k, n_seqs * n, c.n_heads, c.hd, true, &rk))) ||
         (v && (rc = check_rows(ctx, v, n_seqs * n, c.n_heads, c.hd, true, &rv))))
@@ -586,7 +591,8 @@ int qg_kv8_attention_work(qg_ctx *ctx, const qg_kv8 *kv, size_t n_rows, size_t n
     const int rc = check_kv8(ctx, kv);
     if (rc) return rc;
     if (!bytes) return qg_fail(ctx, QG_ERR_INVALID_ARG, "bytes is NULL");
-    if (n_heads == 0 || n_heads % kv->v.n_heads || n_heads > 65535 || n_rows > 0x7FFFFFFFu / (n_heads / kv->v.n_heads))
+    if (n_heads == 0 || n_heads % kv->v.n_heads || n_heads > 65535 || n_rows >= kMostRows ||
+        n_rows * n_heads > 0x7FFFFFFFu)
         return qg_fail(ctx, QG_ERR_SHAPE, "rows or heads");
     *bytes = qg8::attention_work(kv->v, n_rows, n_heads, ctx->n_cu);
     return QG_OK;
@@ -604,7 +610,7 @@ int qg_kv8_attention_dev(qg_ctx *ctx, const qg_kv8 *kv, const qg_batch *batch, s
     if ((rc = check_batch(ctx, kv, batch, &b)) || (rc = check_rows(ctx, q, b.n_rows, n_heads, kv->v.hd, false, &rq)) ||
         (rc = check_rows(ctx, out, b.n_rows, n_heads, kv->v.hd, true, &ro)))
         return rc;
-    if (b.n_rows > 0x7FFFFFFFu / (n_heads / kv->v.n_heads)) return qg_fail(ctx, QG_ERR_SHAPE, "too many rows");
+    if (b.n_rows * n_heads > 0x7FFFFFFFu) return qg_fail(ctx, QG_ERR_SHAPE, "too many rows");
     if (rq.f16 != ro.f16) return qg_fail(ctx, QG_ERR_UNSUPPORTED_TYPE, "q and out of two types");
     if (b.n_rows == 0) return QG_OK;
     const size_t need = qg8::attention_work(kv->v, b.n_rows, n_heads, ctx->n_cu);

@@ -24,8 +24,9 @@
 //     NaN scale reaches the rows that see a position of it.
 //
 // Rows are (token, query head) pairs of one kv head: pair r of a sequence is token
-// r / n_rep, head r % n_rep (the callers keep n_rows * n_rep below 2^31).  Tiles of kM pairs of one sequence and kv head are the
-// items; an item's work is its visible blocks in chunks of a few.  All items'
+// r / n_rep, head r % n_rep (the callers keep n_rows * n_heads below 2^31, and the
+// cache's sequences * heads within 2^26).  Tiles of pairs of one sequence and kv
+// head are the items; an item's work is its visible blocks in chunks of a few.  All items'
 // chunks, end to end, are dealt out evenly to the workgroups (about two per
 // compute unit) whatever the sequences' lengths; a workgroup's share may end
 // inside an item, then the parts' (m, sum, unnormalised output) go to the
@@ -204,17 +205,19 @@ template <uint32_t M> __device__ Order order_of(const Problem &a)
 struct Item {
     uint32_t seq, head, tile, tiles;
     uint32_t start;                     // place of its first chunk
+    uint32_t s0, before;                // its 64 sequences' first, and the places before them
     Tile t;
     Span s;
 };
 
-// The item that holds place `at` (less than the total).
-template <uint32_t M> __device__ Item find(const Problem &a, uint32_t at, const Order &o)
+// The item that holds place `at` (less than the total); `before` places lie
+// before the sequences from s0 on, a multiple of 64, and `at` is none of them.
+template <uint32_t M>
+__device__ Item find(const Problem &a, uint32_t at, const Order &o, uint32_t s0 = 0, uint32_t before = 0)
 {
     const uint32_t lane = threadIdx.x & 63u;
     Item it{};
-    uint32_t before = 0;
-    for (uint32_t s0 = 0; s0 < a.v.n_seqs; s0 += 64) {
+    for (; s0 < a.v.n_seqs; s0 += 64) {
         Span own = o.own;
         const uint32_t c = s0 == 0 ? o.first : scan64(lane_places<M>(a, s0, &own));
         const uint64_t past = __ballot(before + c > at);
@@ -225,6 +228,8 @@ template <uint32_t M> __device__ Item find(const Problem &a, uint32_t at, const 
         const uint32_t l = (uint32_t)__ffsll((unsigned long long)past) - 1;
         const uint32_t up_to = lane_of(c, l), below = l ? lane_of(c, l - 1) : 0u;
         it.seq = s0 + l;
+        it.s0 = s0;
+        it.before = before;
         it.s = span_at(own, l);
         before += below;
         const uint32_t per_head = (up_to - below) / a.v.n_heads;
@@ -260,7 +265,7 @@ template <uint32_t M> __device__ void advance(const Problem &a, Item &it, const 
         it.head++;
         it.tile = 0;
     } else {
-        it = find<M>(a, end, o);
+        it = find<M>(a, end, o, it.s0, it.before);
         return;
     }
     it.start = end + a.lead;

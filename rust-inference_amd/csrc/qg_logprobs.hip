@@ -338,7 +338,8 @@ extern "C" {
 int qg_logprobs_work(qg_ctx *ctx, size_t n_rows, size_t n_cols, size_t k, size_t *bytes)
 {
     if (!ctx || !bytes) return qg_fail(ctx, QG_ERR_INVALID_ARG, "ctx or bytes is NULL");
-    if (n_rows > 0x7FFFFFFFu || n_cols < 1 || n_cols > 0x7FFFFFFFu || k > QG_LOGPROBS_MAX_TOP)
+    // a launch counts its threads in 32 bits, 256 for each row
+    if (n_rows >> 24 || n_cols < 1 || n_cols > 0x7FFFFFFFu || k > QG_LOGPROBS_MAX_TOP)
         return qg_fail(ctx, QG_ERR_SHAPE, "logits or alternatives");
     // what calls of fewer rows need too: parts * rows is largest just before the
     // rows alone are enough workgroups

@@ -131,6 +131,54 @@ def test_many_sequences(rinf, ctx):
     case(rinf, ctx, [int(n) for n in rng.integers(0, 90, 200)], [1] * 200, 4, 1, 64, "f16", seed=6)
 
 
+def test_many_groups_of_sequences(rinf, ctx):
+    """More sequences than a wave looks at together, a workgroup's items in several of those groups."""
+    rng = np.random.default_rng(13)
+    case(rinf, ctx, [int(n) for n in rng.integers(0, 40, 1300)], [int(n) for n in rng.integers(0, 3, 1300)], 2, 1, 16, "f32", seed=7)
+    case(rinf, ctx, [int(n) for n in rng.integers(0, 40, 1100)], [1] * 1100, 1, 1, 16, "f16", seed=8)
+
+
+@pytest.mark.parametrize("heads,n", [(1, 20), (1, 100), (512, 130)])
+def test_f32_has_both_pieces(rinf, ctx, heads, n):
+    """f32 rows against a bound so narrow that a lost low piece of q or of p is
+    past it (tiles of 16, 64 and 128 pairs).  A row has two elements that are not
+    zero, so that its scores add two products (the others add exactly nothing):
+    the bound of `reference` with 2 for hd, over at most 130 positions."""
+    rng = np.random.default_rng(heads + n)
+    hd, nz = 64, 2
+    cache = ctx.kv8(1, heads, hd, n)
+    k, v = (rng.standard_normal((n, heads, hd)).astype(np.float32) for _ in range(2))
+    write(ctx, cache, [k], [v], [n])
+    q = np.zeros((n, heads, hd), np.float32)
+    for h in range(heads):
+        q[:, h, rng.permutation(hd)[:nz]] = rng.uniform(3, 5, (n, nz)) * rng.choice([-1, 1], (n, nz))
+    got = run(ctx, cache, q, [n], [0, n], scale=1.0).astype(np.float64)
+    kq, vq = all_quantised(k).astype(np.float64), all_quantised(v).astype(np.float64)
+    sees = np.tril(np.ones((n, n), bool))
+    past = np.zeros(2)
+    some = range(heads) if heads == 1 else range(0, heads, 37)
+
+    def out(x, h, rounded):
+        s = np.where(sees, x @ kq[:, h].T, -np.inf)
+        e = np.exp(s - s.max(1, keepdims=True))
+        p = e.astype(np.float16).astype(np.float64) if rounded else e
+        return p @ vq[:, h] / e.sum(1, keepdims=True), s
+
+    for h in some:
+        x = q[:, h].astype(np.float64)
+        want, s = out(x, h, False)
+        a = (np.abs(x) @ np.abs(kq[:, h]).T * sees).max(1, keepdims=True)
+        tol = np.abs(vq[:, h]).max() * (2 * (nz + 8) * a + n / 32 + 80) * U
+        assert (np.abs(got[:, h] - want) <= tol).all(), (h, (np.abs(got[:, h] - want) / tol).max())
+        past[0] += (np.abs(out(x.astype(np.float16).astype(np.float64), h, False)[0] - want) > tol).any(1).mean()
+        past[1] += (np.abs(out(x, h, True)[0] - want) > tol).any(1).mean()
+    # without either low piece rows would be past their bounds (one is enough to
+    # fail; a row that sees one position hides its score, and here the largest
+    # weight, 1, has no low piece)
+    assert (past > 0).all(), past
+    cache.free()
+
+
 def test_scales(rinf, ctx):
     """Scores that spread far, that all are equal, and a negative scale."""
     for scale in (0.0, 1.0, -0.3, 30.0):
@@ -334,6 +382,10 @@ def test_refusals(rinf, ctx):
         assert call(size=n.value - 1) == 7 and call(w=None) == 1 and call(w=work.data_ptr() + 4) == 1
     assert lib.qg_kv8_attention_work(ctx.h, cache.h, 2, 3, ctypes.byref(n)) == 7
     assert lib.qg_kv8_attention_work(ctx.h, cache.h, 1 << 31, 4, ctypes.byref(n)) == 7
+    assert lib.qg_kv8_attention_work(ctx.h, cache.h, 1 << 28, 2, ctypes.byref(n)) == 7
+    assert lib.qg_kv8_attention_work(ctx.h, cache.h, 1 << 27, 16, ctypes.byref(n)) == 7       # 2^31 rows of heads
+    assert call(b=rinf.Batch(1 << 28, lens.data_ptr(), lens.data_ptr()), ro=rinf.Rows(out.data_ptr(), 0, 256, 64)) == 7
+    assert call(heads=16, b=rinf.Batch(1 << 27, lens.data_ptr(), lens.data_ptr()), ro=rinf.Rows(out.data_ptr(), 0, 1024, 64)) == 7
     assert lib.qg_kv8_attention_work(ctx.h, cache.h, 2, 4, None) == 1
     torch.cuda.synchronize()
     cache.free()

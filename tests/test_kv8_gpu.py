@@ -357,6 +357,8 @@ def test_refusals(rinf, ctx):
     assert call(b=rinf.Batch(3, None, lens.data_ptr())) == 7                      # one row per sequence
     assert call(b=rinf.Batch(2, None, None)) == 1 and call(b=rinf.Batch(2, None, lens.data_ptr() + 1)) == 1
     assert call(b=rinf.Batch(1 << 31, lens.data_ptr(), lens.data_ptr())) == 7
+    assert call(b=rinf.Batch(1 << 28, lens.data_ptr(), lens.data_ptr())) == 7
+    assert lib.qg_kv8_create(ctx.h, 8193, 8192, 1, 1, ctypes.byref(h)) == 7
     assert lib.qg_kv8_write_dev(ctx.h, cache.h, None, None, None, None) == 1
     out = rows_()
     read_ = lambda *a, o=out: lib.qg_kv8_read_dev(ctx.h, cache.h, *a, ctypes.byref(o), None, None)  # noqa: E731

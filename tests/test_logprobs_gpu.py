@@ -228,6 +228,7 @@ def test_refusals(rinf, ctx):
     assert f(x=None) == 1 and f(t=None) == 1 and f(lp=None) == 1 and f(ids=None) == 1 and f(tl=None) == 1
     assert f(x=p + 2) == 1 and f(ent=q + 1) == 1 and f(tl=q + 2) == 1
     assert f(cols=0) == 7 and f(ld=99) == 7 and f(k=65) == 7 and f(cols=1 << 31, ld=1 << 31) == 7 and f(rows=1 << 31) == 7
+    assert f(rows=1 << 24) == 7
     assert f(ld=1 << 62) == 7
     assert lib.qg_logprobs_work(ctx.h, 1, 1, 1, None) == 1 and lib.qg_logprobs_work(None, 1, 1, 1, ctypes.byref(n)) == 1
     with pytest.raises(rinf.QgemvError):

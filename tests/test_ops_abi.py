@@ -6,6 +6,7 @@ from __future__ import annotations
 import ctypes
 import pathlib
 import re
+from unittest import mock
 
 import pytest
 
@@ -46,3 +47,22 @@ def test_layout_is_one_to_one(dp):
     key, value = _function("key_at"), _function("value_at")
     for f in (lambda t, d: key(t, d, dp), value):
         assert sorted(f(t, d) for t in range(32) for d in range(dp)) == list(range(32 * dp))
+
+
+def test_tensors_of_another_device(rinf):
+    """Host tensors are refused before their addresses reach the library."""
+    import torch
+
+    class Context:                                # no device, and a library that is not to be called
+        device, h, lib = 0, None, mock.MagicMock()
+        logprobs_dev = rinf.GpuContext.logprobs_dev
+
+    cache = rinf.Kv8Cache(Context(), None, 1, 1, 64, 32)
+    x, lens = torch.zeros(1, 1, 64), torch.ones(1, dtype=torch.int32)
+    for call in (lambda: cache.write_dev(x, x, lens), lambda: cache.attention_dev(x, x, lens),
+                 lambda: cache.read_dev(0, 1, 0, 1, x, x),
+                 lambda: Context().logprobs_dev(x[0], lens.view(1, 1), x[0, :, :1])):
+        with pytest.raises(rinf.QgemvError, match="device"):
+            call()
+    for f in ("qg_kv8_write_dev", "qg_kv8_attention_dev", "qg_kv8_read_dev", "qg_logprobs_dev"):
+        assert not getattr(Context.lib, f).called
