@@ -22,6 +22,7 @@ import ctypes
 import os
 import pathlib
 import re
+import struct
 
 HERE = pathlib.Path(__file__).resolve().parent
 LIB_PATH = HERE / "libqgemv.so"
@@ -401,8 +402,10 @@ class GpuContext:
 
 
 # The calls of include/qgops.h come once per layer and token, so their wrappers
-# keep to what a call needs (addresses as plain integers, one look at a tensor's
-# shape and strides).
+# keep to what a call needs: addresses as plain integers, one look at a tensor's
+# shape and strides, and qg_batch and two qg_rows packed into a buffer of the
+# cache's (3.8 and 5.3 us a write and an attention call on the host, 5.0 and 6.4
+# with ctypes structures; the smallest attention kernel takes 6).
 
 def _addr(t, dev: int, what: str):
     """Address of a tensor on the context's device; None stays None."""
@@ -418,6 +421,7 @@ def _nbytes(t) -> int:
 
 
 _row_types: dict = {}
+_ARGS = struct.Struct("@NPPPINNPINN")      # qg_batch, qg_rows, qg_rows
 
 
 def _row_type(t) -> int:
@@ -428,21 +432,27 @@ def _row_type(t) -> int:
     return _row_types.get(t.dtype, 0xFFFFFFFF)
 
 
-def _words(t, n: int, dev: int, what: str):
-    """Address of n contiguous 4-byte values."""
+def _words(t, n: int, dev: int, what: str) -> int:
+    """Address of n contiguous 4-byte values; 0 for None."""
     if t is None:
-        return None
-    if t.numel() != n or t.dtype.itemsize != 4 or not t.is_contiguous():
+        return 0
+    if t.numel() != n or t.element_size() != 4 or not t.is_contiguous():
         raise QgemvError(7, f"{what}: {n} contiguous values of 4 bytes")
-    return _addr(t, dev, what)
+    if t.get_device() != dev:
+        raise QgemvError(1, f"{what}: a tensor on the context's device")
+    return t.data_ptr()
 
 
-def _rows(t, n_rows: int, heads: int, hd: int, dev: int, what: str) -> Rows:
-    """qg_rows of a torch tensor [rows, heads, head_dim]."""
-    s = t.stride()
-    if t.shape != (n_rows, heads, hd) or (s[2] != 1 and hd > 1):
-        raise QgemvError(7, f"{what} is not [{n_rows}, {heads}, {hd}] with contiguous elements")
-    return Rows(_addr(t, dev, what), _row_type(t), s[0], s[1])
+def _rows(t, shape, dev: int, what: str):
+    """What qg_rows holds for a torch tensor [rows, heads, head_dim]; nothing for None."""
+    if t is None:
+        return 0, 0, 0, 0
+    ld_row, ld_head, step = t.stride() if t.dim() == 3 else (0, 0, 0)
+    if t.shape != shape or (step != 1 and shape[2] > 1):
+        raise QgemvError(7, f"{what} is not {list(shape)} with contiguous elements")
+    if t.get_device() != dev:
+        raise QgemvError(1, f"{what}: a tensor on the context's device")
+    return t.data_ptr(), _row_type(t), ld_row, ld_head
 
 
 class Kv8Cache:
@@ -452,6 +462,9 @@ class Kv8Cache:
     def __init__(self, ctx: GpuContext, h, n_seqs: int, n_kv_heads: int, head_dim: int, max_len: int):
         self.ctx, self.h = ctx, h
         self.n_seqs, self.n_kv_heads, self.head_dim, self.max_len = n_seqs, n_kv_heads, head_dim, max_len
+        self._args = ctypes.create_string_buffer(_ARGS.size)
+        at = ctypes.addressof(self._args)
+        self._batch, self._rows0, self._rows1 = _P(at), _P(at + 24), _P(at + 56)
 
     def free(self):
         # a closed context has already freed its caches (qg_destroy)
@@ -471,29 +484,27 @@ class Kv8Cache:
         self.ctx.check(self.ctx.lib.qg_kv8_info(self.h, None, None, None, None, ctypes.byref(n)), "qg_kv8_info")
         return n.value
 
-    def _batch(self, n_rows: int, lens, starts) -> Batch:
-        dev = self.ctx.device
-        return Batch(n_rows, _words(starts, self.n_seqs + 1, dev, "starts"), _words(lens, self.n_seqs, dev, "lens"))
-
     def write_dev(self, k, v, lens, starts=None, stream=None):
         """Cache k and v [rows, n_kv_heads, head_dim]; lens: every sequence's
         positions with these rows (qg_kv8_write_dev)."""
-        n, heads, hd, dev = k.shape[0], self.n_kv_heads, self.head_dim, self.ctx.device
-        rc = self.ctx.lib.qg_kv8_write_dev(self.ctx.h, self.h, ctypes.byref(self._batch(n, lens, starts)),
-                                           ctypes.byref(_rows(k, n, heads, hd, dev, "k")),
-                                           ctypes.byref(_rows(v, n, heads, hd, dev, "v")), stream or None)
+        ctx, n, n_seqs = self.ctx, k.shape[0], self.n_seqs
+        dev, shape = ctx.device, (n, self.n_kv_heads, self.head_dim)
+        _ARGS.pack_into(self._args, 0, n, _words(starts, n_seqs + 1, dev, "starts"), _words(lens, n_seqs, dev, "lens"),
+                        *_rows(k, shape, dev, "k"), *_rows(v, shape, dev, "v"))
+        rc = ctx.lib.qg_kv8_write_dev(ctx.h, self.h, self._batch, self._rows0, self._rows1, stream or None)
         if rc:
-            self.ctx.check(rc, "qg_kv8_write_dev")
+            ctx.check(rc, "qg_kv8_write_dev")
 
     def read_dev(self, seq: int, n_seqs: int, pos: int, n: int, k=None, v=None, stream=None):
         """Positions pos .. pos + n of n_seqs sequences from seq on as values
         [n_seqs * n, n_kv_heads, head_dim] (qg_kv8_read_dev)."""
-        r, heads, hd, dev = n_seqs * n, self.n_kv_heads, self.head_dim, self.ctx.device
-        rc = self.ctx.lib.qg_kv8_read_dev(self.ctx.h, self.h, seq, n_seqs, pos, n,
-                                          None if k is None else ctypes.byref(_rows(k, r, heads, hd, dev, "k")),
-                                          None if v is None else ctypes.byref(_rows(v, r, heads, hd, dev, "v")), stream or None)
+        ctx = self.ctx
+        dev, shape = ctx.device, (n_seqs * n, self.n_kv_heads, self.head_dim)
+        _ARGS.pack_into(self._args, 0, 0, 0, 0, *_rows(k, shape, dev, "k"), *_rows(v, shape, dev, "v"))
+        rc = ctx.lib.qg_kv8_read_dev(ctx.h, self.h, seq, n_seqs, pos, n, None if k is None else self._rows0,
+                                     None if v is None else self._rows1, stream or None)
         if rc:
-            self.ctx.check(rc, "qg_kv8_read_dev")
+            ctx.check(rc, "qg_kv8_read_dev")
 
     def attention_work(self, n_rows: int, n_heads: int) -> int:
         """Bytes of workspace attention_dev needs (qg_kv8_attention_work)."""
@@ -505,13 +516,16 @@ class Kv8Cache:
     def attention_dev(self, q, out, lens, work=None, starts=None, scale=None, window: int = 0, stream=None):
         """out = attention of q [rows, n_heads, head_dim] over the cache; scale:
         1 / sqrt(head_dim) by default (qg_kv8_attention_dev)."""
-        n, heads, hd, dev = q.shape[0], q.shape[1], self.head_dim, self.ctx.device
-        rc = self.ctx.lib.qg_kv8_attention_dev(
-            self.ctx.h, self.h, ctypes.byref(self._batch(n, lens, starts)), heads, ctypes.byref(_rows(q, n, heads, hd, dev, "q")),
-            hd ** -0.5 if scale is None else scale, window, ctypes.byref(_rows(out, n, heads, hd, dev, "out")),
-            _addr(work, dev, "work"), _nbytes(work), stream or None)
+        ctx, n_seqs, hd = self.ctx, self.n_seqs, self.head_dim
+        n, heads = q.shape[:2]
+        dev, shape = ctx.device, (n, heads, hd)
+        _ARGS.pack_into(self._args, 0, n, _words(starts, n_seqs + 1, dev, "starts"), _words(lens, n_seqs, dev, "lens"),
+                        *_rows(q, shape, dev, "q"), *_rows(out, shape, dev, "out"))
+        rc = ctx.lib.qg_kv8_attention_dev(ctx.h, self.h, self._batch, heads, self._rows0,
+                                          hd ** -0.5 if scale is None else scale, window, self._rows1,
+                                          _addr(work, dev, "work"), _nbytes(work), stream or None)
         if rc:
-            self.ctx.check(rc, "qg_kv8_attention_dev")
+            ctx.check(rc, "qg_kv8_attention_dev")
 
 
 class DeviceMatrix:
