@@ -101,6 +101,32 @@ __device__ __forceinline__ int code_of(float x, float s, float inv)
     return (int)q;
 }
 
+// The codes of 16 elements as bytes (code + 128), s > 0.  The product's integer is
+// the low byte of its sum with 1.5 2^23 + 128 (rounded once, ties to even); where
+// any remainder reaches s / 2, code_of decides for all of them.
+__device__ __forceinline__ uint4 codes_of(const float *x, float s, float inv)
+{
+    constexpr float kMagic = 12582912.f + (float)kZero;
+    const float h = 0.5f * s;
+    float most = 0.f;
+    union { uint32_t w[4]; uint8_t b[16]; uint4 u; } r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t t[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float y = __builtin_fmaf(x[4 * i + j], inv, kMagic);
+            most = fmaxf(most, fabsf(__builtin_fmaf(kMagic - y, s, x[4 * i + j])));
+            t[j] = __float_as_uint(y);
+        }
+        const uint32_t lo = __builtin_amdgcn_perm(t[1], t[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(t[3], t[2], 0x04000C0Cu);
+        r.w[i] = lo | hi;
+    }
+    if (most >= h)
+        for (int j = 0; j < 16; j++) r.b[j] = (uint8_t)(code_of(x[j], s, inv) + kZero);
+    return r.u;
+}
+
 constexpr uint32_t kInf = 0x7F800000u;
 
 // Block `b`'s positions lo .. hi (of 32) from the rows, those before lo from
@@ -119,7 +145,8 @@ __device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint6
     float val[NC][16];
     const bool fresh = t >= lo && t < hi, old = t < lo;
     const float s_old = lo ? *scale : 0.f;
-    uint32_t m = 0;
+    uint32_t m;
+    float top = 0.f;
 #pragma unroll
     for (int i = 0; i < NC; i++) {
         const uint32_t d = 16u * (c + 8u * i);
@@ -136,8 +163,9 @@ __device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint6
                 }
         }
 #pragma unroll
-        for (int j = 0; j < 16; j++) m = max(m, __float_as_uint(val[i][j]) & 0x7FFFFFFFu);
+        for (int j = 0; j < 16; j++) top = __builtin_elementwise_maximum(top, fabsf(val[i][j]));    // NaN if any is
     }
+    m = __float_as_uint(top) & 0x7FFFFFFFu;
     // a position's largest magnitude, over its eight threads
     m = max(m, (uint32_t)__shfl_xor((int)m, 1, 64));
     m = max(m, (uint32_t)__shfl_xor((int)m, 2, 64));
@@ -174,9 +202,7 @@ __device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint6
         if (d >= dp) break;
         union { uint8_t b[16]; uint4 u; } w;
         w.u = make_uint4(kZeros, kZeros, kZeros, kZeros);
-        if (s > 0.f && put)
-#pragma unroll
-            for (int j = 0; j < 16; j++) w.b[j] = (uint8_t)(code_of(val[i][j], s, inv) + kZero);
+        if (s > 0.f && put) w.u = codes_of(val[i], s, inv);
         if (key) {
             if (put) *(uint4 *)(codes + key_at(t, d, dp)) = w.u;
         } else if (whole) {
@@ -196,15 +222,17 @@ __device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint6
         // 16 bytes of the layout at a time: two elements at eight positions
         for (uint32_t u = tid; u < 2 * dp; u += 256) {
             const uint32_t g = u >> 4 & 3u, d = (u >> 6) * 32u + 2u * (u & 15u);
-            union { uint8_t b[16]; uint4 u; } w;
+            uint32_t two[8], w[4];
 #pragma unroll
-            for (uint32_t j = 0; j < 8; j++) {
-                const uint32_t p = 4u * g + (j & 3u) + (j >> 2) * 16u;
-                const uint16_t two = *(const uint16_t *)(stage + p * (dp + 16) + d);
-                w.b[j] = (uint8_t)two;
-                w.b[8 + j] = (uint8_t)(two >> 8);
+            for (uint32_t j = 0; j < 8; j++)
+                two[j] = *(const uint16_t *)(stage + (4u * g + (j & 3u) + (j >> 2) * 16u) * (dp + 16) + d);
+#pragma unroll
+            for (uint32_t j = 0; j < 2; j++) {            // four positions: their first elements, their second ones
+                const uint32_t a = two[4 * j] | two[4 * j + 1] << 16, b = two[4 * j + 2] | two[4 * j + 3] << 16;
+                w[j] = __builtin_amdgcn_perm(b, a, 0x06040200u);
+                w[2 + j] = __builtin_amdgcn_perm(b, a, 0x07050301u);
             }
-            *(uint4 *)(codes + u * 16u) = w.u;
+            *(uint4 *)(codes + u * 16u) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
     if (tid == 0) *scale = s;
@@ -213,8 +241,11 @@ __device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint6
 }
 
 // Grid: (items, heads, keys / values).  Bound by the latency of a few dependent
-// loads; WAVES: workgroups of which a compute unit holds at least so many (fewer
-// registers for each).
+// loads where there is little (one token 4.6 us, 1001 tokens of 8 heads of 128 in
+// f32 8.4), by the memory where there is much (32 prompts of up to 2048 tokens,
+// f16, 62 us: 3 bytes an element at 3.2 to 6.4 TB/s by how much of the input the last level
+// cache holds); WAVES: workgroups of which a compute unit holds at least so many
+// (fewer registers for each).
 //
 // The scale of a block follows from its largest magnitude, so a new token in a
 // block that is partly there costs its own row and 32 remembered magnitudes

@@ -562,7 +562,17 @@ __device__ __forceinline__ uint32_t place_of(uint32_t id, uint32_t n)
 
 // Few rows: tiles of 16 pairs.  The four waves take an item's blocks in turn, each
 // with all 16 rows and operands straight from the cache (the next block's 64 dp
-// bytes are requested before a block is used); their sums are joined in LDS.
+// bytes are requested before a block is used); their sums are joined in LDS.  A
+// part's fixed cost (its rows, the first loads, the join) hides behind the next
+// part's loads, which are requested before the join.
+//
+// Bound by the read of the cache where it is long: 64 sequences of up to 8192
+// tokens, 8 kv heads of 128, f16 rows 117 us (the 0.55 GB of codes at 4.7 TB/s; a
+// large copy does 5.0), one of 131072 tokens 47 (5.7 TB/s, half of it from the last
+// level cache).  Short ones are a chain of latencies: lengths, codes, products,
+// join, about 11000 cycles at 49 tokens (6.1 us), 17400 at 2256 (10.6 with four
+// kv heads of 18 parts each).  Two workgroups a compute unit; three (with half
+// the registers) were slower, and so were parts of 8 or 16 blocks.
 constexpr uint32_t kFewM = 16;
 
 template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) few_k(Problem a)
@@ -753,6 +763,16 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
 // work at the same time: the scores of block j + 1 while block j's are turned
 // into weights, the outputs of block j while the codes of block j + 2 are turned
 // into f16.
+//
+// Bound by the matrix cores and the vector units together (16 of the latter's
+// instructions a block and tile are exponentials): 1001 tokens of 32 heads of 128
+// in f32, two pieces of q and p, 43 us, 0.19 PFLOP/s of the formula and twice that
+// of products; 2048 new tokens of four sequences in f16 over 4096 positions each
+// 440 us, 0.70 PFLOP/s, where a large f16 matrix product does 1.11: matrix cores
+// busy in 31 % of the cycles, vector units in 42 %, waves waiting (data, barriers)
+// in 30 % of theirs.  Two workgroups of 48 KB a compute unit; larger tiles (256
+// pairs) spill: 744 against 480 us at that stage.  Rows that take 16-byte accesses
+// go straight from and to memory; through LDS they cost a part 10000 cycles more.
 template <int DP, int NP, int RT> __global__ void __launch_bounds__(256, 2) many_k(Problem a)
 {
     constexpr uint32_t M = 64 * RT;
@@ -1003,7 +1023,8 @@ template <int DP, int NP, int RT> __global__ void __launch_bounds__(256, 2) many
 // in slot 1, the others' in slot 0).  Grid: (workgroups - 1, row groups); the
 // workgroup of the second part does it.  DP / 4 lanes take a row's elements; few
 // rows of many parts (PARTS): the other threads take parts in turn; else they
-// take rows.
+// take rows.  Bound by its launch and two dependent reads: 4 us behind few_k, 6.8
+// and 14 behind many_k's tiles of 64 and 128 pairs (up to 67 MB of parts).
 template <uint32_t M, int DP, bool PARTS> __global__ void __launch_bounds__(256) merge_k(Problem a)
 {
     constexpr uint32_t L = DP / 4, N = 256 / L;            // 192 / 4 = 48: 5 groups, 16 lanes idle

@@ -23,8 +23,10 @@ namespace {
 // candidates leave the registers, usually little more than k; they are ranked by
 // counting the larger ones.
 //
-// Bound by the read of the logits where there are many rows, by two dependent
-// launches where there are few.
+// Bound by the read of the logits where there are many rows (2048 rows of 151936
+// in f16, no alternatives: 152 us, 4.1 TB/s, what a plain sum of them reads at), by
+// two dependent launches where there are few: one row of 152064 with 8 alternatives
+// 8.8 us and 7.3 (64 of them: 9.8 and 15.2), 64 rows of 128256 with 20 14.0 and 5.2.
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kMaxParts = 64, kMaxK = QG_LOGPROBS_MAX_TOP;
 constexpr float kLowest = -3.402823466e38f, kLog2e = 1.44269504f, kLn2 = 0.693147181f;
