@@ -18,13 +18,13 @@ __device__ __forceinline__ uint32_t wave_max_u(uint32_t v)
 // What a call does to one sequence: the positions first .. last of blocks b0 ..
 // bl.  Items are what one workgroup per head takes: item 0 block b0 and, where
 // the last block stays open, that one too (they share the f32 tail); item j >
-// 0 the whole block b0 + j.
+// 0 the `group` whole blocks from b0 + 1 + (j - 1) group on.
 struct Piece {
     Span s;
     uint32_t first, end, b0, bl, items;   // positions first .. end
 };
 
-__device__ __forceinline__ Piece piece_of(const Batch &b, uint32_t seq, uint32_t max_len)
+__device__ __forceinline__ Piece piece_of(const Batch &b, uint32_t seq, uint32_t max_len, uint32_t group)
 {
     Piece p;
     p.s = span_of(b, seq);
@@ -34,7 +34,8 @@ __device__ __forceinline__ Piece piece_of(const Batch &b, uint32_t seq, uint32_t
     if (p.s.n == 0 || p.first >= p.end) return p;
     p.b0 = p.first / kBlock;
     p.bl = (p.end - 1) / kBlock;
-    p.items = p.bl - p.b0 + ((p.bl > p.b0 && p.end % kBlock) ? 0u : 1u);
+    const uint32_t whole = p.bl - p.b0 - ((p.bl > p.b0 && p.end % kBlock) ? 1u : 0u);
+    p.items = 1 + (whole + group - 1) / group;
     return p;
 }
 
@@ -46,20 +47,20 @@ __device__ __forceinline__ uint32_t lane_of(uint32_t v, uint32_t l)
 // The sequence, its piece and the item of workgroup `want`: the items of the
 // sequences before it are counted 64 sequences at a time, by every wave on its
 // own.  False behind the last item.
-__device__ bool find_item(const Batch &b, uint32_t n_seqs, uint32_t max_len, uint32_t want, uint32_t *seq,
-                          uint32_t *item, Piece *piece)
+__device__ bool find_item(const Batch &b, uint32_t n_seqs, uint32_t max_len, uint32_t group, uint32_t want,
+                          uint32_t *seq, uint32_t *item, Piece *piece)
 {
     const uint32_t lane = threadIdx.x & 63u;
     if (b.lens && !b.starts) {                       // one row each
         *seq = want;
         *item = 0;
-        *piece = piece_of(b, want, max_len);
+        *piece = piece_of(b, want, max_len, group);
         return piece->items != 0;
     }
     uint32_t before = 0;
     for (uint32_t s0 = 0; s0 < n_seqs; s0 += 64) {
         Piece p{};
-        if (s0 + lane < n_seqs) p = piece_of(b, s0 + lane, max_len);
+        if (s0 + lane < n_seqs) p = piece_of(b, s0 + lane, max_len, group);
         uint32_t n = p.items;
 #pragma unroll
         for (uint32_t o = 1; o < 64; o <<= 1) {
@@ -129,13 +130,40 @@ __device__ __forceinline__ uint4 codes_of(const float *x, float s, float inv)
 
 constexpr uint32_t kInf = 0x7F800000u;
 
+// A block's scale from the bits of its largest magnitude.
+__device__ __forceinline__ float scale_of(uint32_t m)
+{
+    const float s = __uint_as_float(m) / 127.0f;
+    return m >= kInf ? __uint_as_float(0x7FC00000u) : s < 0x1p-126f ? 0.f : s;
+}
+
+// Values of a block from LDS (rows of dp + 16 bytes) into the cache's order, 16
+// bytes at a time: two elements at eight positions.
+__device__ __forceinline__ void put_values(const uint8_t *stage, uint8_t *codes, uint32_t dp)
+{
+    for (uint32_t u = threadIdx.x; u < 2 * dp; u += 256) {
+        const uint32_t g = u >> 4 & 3u, d = (u >> 6) * 32u + 2u * (u & 15u);
+        uint32_t two[8], w[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++)
+            two[j] = *(const uint16_t *)(stage + (4u * g + (j & 3u) + (j >> 2) * 16u) * (dp + 16) + d);
+#pragma unroll
+        for (uint32_t j = 0; j < 2; j++) {                // four positions: their first elements, their second ones
+            const uint32_t a = two[4 * j] | two[4 * j + 1] << 16, b = two[4 * j + 2] | two[4 * j + 3] << 16;
+            w[j] = __builtin_amdgcn_perm(b, a, 0x06040200u);
+            w[2 + j] = __builtin_amdgcn_perm(b, a, 0x07050301u);
+        }
+        *(uint4 *)(codes + u * 16u) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
 // Block `b`'s positions lo .. hi (of 32) from the rows, those before lo from
 // what the cache holds.  One workgroup of 256: thread (t, c): position t =
 // tid / 8, elements 16 (c + 8 i) .. + 16.
 template <int NC>
-__device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint64_t ld_row, uint32_t sh, uint64_t base,
-                            uint32_t b, uint32_t lo, uint32_t hi, int slot, bool held, bool open, bool key,
-                            uint32_t *maxes, uint32_t *red, uint8_t *stage)
+__device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint64_t base, uint32_t b, uint32_t lo,
+                            uint32_t hi, int slot, bool held, bool open, bool key, uint32_t *maxes, uint32_t *red,
+                            uint8_t *stage)
 {
     const uint32_t tid = threadIdx.x, t = tid >> 3, c = tid & 7u, dp = v.dp;
     uint8_t *codes = v.codes + (base * v.n_blocks + b) * kBlock * dp;
@@ -152,7 +180,7 @@ __device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint6
         const uint32_t d = 16u * (c + 8u * i);
         if (d >= dp) break;
         if (fresh) {
-            load16(x, row_at + (uint64_t)(t - lo) * ld_row, d, v.hd, val[i]);
+            load16(x, row_at + (uint64_t)(t - lo) * x.ld_row, d, v.hd, val[i]);
         } else {
 #pragma unroll
             for (int j = 0; j < 16; j++) val[i][j] = 0.f;
@@ -176,9 +204,7 @@ __device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint6
     if ((tid & 63u) == 0) red[tid >> 6] = m;
     __syncthreads();
     m = max(max(red[0], red[1]), max(red[2], red[3]));
-    float s = __uint_as_float(m) / 127.0f;
-    if (s < 0x1p-126f) s = 0.f;
-    if (m >= kInf) s = __uint_as_float(0x7FC00000u);
+    const float s = scale_of(m);
     const float inv = s > 0.f ? 1.0f / s : 0.f;              // NaN: no codes
     // the block's codes of the positions before lo stand while the scale does
     const bool again = lo > 0 && (__float_as_uint(s) != __float_as_uint(s_old) || !held);
@@ -219,46 +245,130 @@ __device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint6
     }
     if (!key && whole) {
         __syncthreads();
-        // 16 bytes of the layout at a time: two elements at eight positions
-        for (uint32_t u = tid; u < 2 * dp; u += 256) {
-            const uint32_t g = u >> 4 & 3u, d = (u >> 6) * 32u + 2u * (u & 15u);
-            uint32_t two[8], w[4];
-#pragma unroll
-            for (uint32_t j = 0; j < 8; j++)
-                two[j] = *(const uint16_t *)(stage + (4u * g + (j & 3u) + (j >> 2) * 16u) * (dp + 16) + d);
-#pragma unroll
-            for (uint32_t j = 0; j < 2; j++) {            // four positions: their first elements, their second ones
-                const uint32_t a = two[4 * j] | two[4 * j + 1] << 16, b = two[4 * j + 2] | two[4 * j + 3] << 16;
-                w[j] = __builtin_amdgcn_perm(b, a, 0x06040200u);
-                w[2 + j] = __builtin_amdgcn_perm(b, a, 0x07050301u);
-            }
-            *(uint4 *)(codes + u * 16u) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        put_values(stage, codes, dp);
     }
     if (tid == 0) *scale = s;
     if (open && tid < hi && (tid >= lo || !held)) tail_max[tid] = maxes[tid];
     __syncthreads();
 }
 
+// A thread's 16 elements of a row as they lie in memory: f16 in two words, else
+// as f32.
+struct Raw {
+    uint4 w[4];
+};
+
+__device__ __forceinline__ Raw load_raw(const Rows &x, uint64_t at, uint32_t d, uint32_t hd)
+{
+    Raw r;
+    if (x.vec) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) r.w[i] = make_uint4(0, 0, 0, 0);
+        if (d >= hd) return r;
+        const uint4 *p = (const uint4 *)((const char *)x.p + (at + d) * (x.f16 ? 2 : 4));
+        r.w[0] = p[0];
+        r.w[1] = p[1];
+        if (!x.f16) {
+            r.w[2] = p[2];
+            r.w[3] = p[3];
+        }
+    } else {
+        union { float f[16]; uint4 w[4]; } u;
+        load16(x, at, d, hd, u.f);
+#pragma unroll
+        for (int i = 0; i < 4; i++) r.w[i] = u.w[i];
+    }
+    return r;
+}
+
+__device__ __forceinline__ void floats_of(const Rows &x, const Raw &r, float *y)
+{
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+    if (x.vec && x.f16) {
+        const h8 a = __builtin_bit_cast(h8, r.w[0]), b = __builtin_bit_cast(h8, r.w[1]);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            y[i] = (float)a[i];
+            y[8 + i] = (float)b[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            y[4 * i] = __uint_as_float(r.w[i].x); y[4 * i + 1] = __uint_as_float(r.w[i].y);
+            y[4 * i + 2] = __uint_as_float(r.w[i].z); y[4 * i + 3] = __uint_as_float(r.w[i].w);
+        }
+    }
+}
+
+// `count` whole blocks from b on (rows from element row_at on): nothing of them is
+// kept but codes and scales.  The next block's rows are on their way while one is
+// worked on.  red: two sets in turn, so that a block of keys takes one barrier.
+template <int NC>
+__device__ void write_whole(const View &v, const Rows &x, uint64_t row_at, uint64_t base, uint32_t b, uint32_t count, bool key,
+                            uint32_t (*red)[4], uint8_t *stage)
+{
+    const uint32_t tid = threadIdx.x, t = tid >> 3, c = tid & 7u, dp = v.dp;
+    uint8_t *codes = v.codes + (base * v.n_blocks + b) * kBlock * dp;
+    float *scale = v.scale + base * v.n_blocks + b;
+    const uint64_t at = row_at + (uint64_t)t * x.ld_row;
+    Raw raw[NC];
+#pragma unroll
+    for (int i = 0; i < NC; i++)
+        if (16u * (c + 8u * i) < dp) raw[i] = load_raw(x, at, 16u * (c + 8u * i), v.hd);
+    for (uint32_t k = 0; k < count; k++) {
+        float val[NC][16], top = 0.f;
+#pragma unroll
+        for (int i = 0; i < NC; i++) {
+            if (16u * (c + 8u * i) >= dp) break;
+            floats_of(x, raw[i], val[i]);
+#pragma unroll
+            for (int j = 0; j < 16; j++) top = __builtin_elementwise_maximum(top, fabsf(val[i][j]));    // NaN if any is
+        }
+        if (k + 1 < count)
+#pragma unroll
+            for (int i = 0; i < NC; i++)
+                if (16u * (c + 8u * i) < dp)
+                    raw[i] = load_raw(x, at + (uint64_t)(k + 1) * kBlock * x.ld_row, 16u * (c + 8u * i), v.hd);
+        uint32_t m = wave_max_u(__float_as_uint(top) & 0x7FFFFFFFu);
+        if ((tid & 63u) == 0) red[k & 1u][tid >> 6] = m;
+        __syncthreads();
+        m = max(max(red[k & 1u][0], red[k & 1u][1]), max(red[k & 1u][2], red[k & 1u][3]));
+        const float s = scale_of(m), inv = s > 0.f ? 1.0f / s : 0.f;
+#pragma unroll
+        for (int i = 0; i < NC; i++) {
+            const uint32_t d = 16u * (c + 8u * i);
+            if (d >= dp) break;
+            const uint4 w = s > 0.f ? codes_of(val[i], s, inv) : make_uint4(kZeros, kZeros, kZeros, kZeros);
+            if (key) *(uint4 *)(codes + key_at(t, d, dp)) = w;
+            else *(uint4 *)(stage + t * (dp + 16) + d) = w;
+        }
+        if (!key) {
+            __syncthreads();
+            put_values(stage, codes, dp);
+        }
+        if (tid == 0) scale[k] = s;
+        codes += kBlock * dp;
+    }
+}
+
 // Grid: (items, heads, keys / values).  Bound by the latency of a few dependent
-// loads where there is little (one token 4.6 us, 1001 tokens of 8 heads of 128 in
-// f32 8.4), by the memory where there is much (32 prompts of up to 2048 tokens,
-// f16, 62 us: 3 bytes an element at 3.2 to 6.4 TB/s by how much of the input the last level
-// cache holds); WAVES: workgroups of which a compute unit holds at least so many
-// (fewer registers for each).
+// loads where there is little (one token 4.2 us, 1001 tokens of 8 heads of 128 in
+// f32 7.7), by the memory and its latency where there is much (32 prompts of up to
+// 2048 tokens, 8 heads of 128 in f16, 194 MB: 54 us, 3.6 TB/s).
 //
 // The scale of a block follows from its largest magnitude, so a new token in a
 // block that is partly there costs its own row and 32 remembered magnitudes
 // while it is not the largest, and the block's f32 rows (kept in one of two
 // slots) when it is.  Two slots, because a call that ends one block and opens
 // another must leave the values of the first: the same call may come again.
-template <int NC, int WAVES> __global__ void __launch_bounds__(256, WAVES) write_k(View v, Batch b, Rows k, Rows val)
+template <int NC>
+__global__ void __launch_bounds__(256, NC == 1 ? 5 : 2) write_k(View v, Batch b, Rows k, Rows val, uint32_t group)
 {
-    __shared__ uint32_t maxes[kBlock], red[4];
+    __shared__ uint32_t maxes[kBlock], red[2][4];
     __shared__ __attribute__((aligned(16))) uint8_t stage[kBlock * (128 * NC + 16)];
     uint32_t seq, item;
     Piece p;
-    if (!find_item(b, v.n_seqs, v.max_len, blockIdx.x, &seq, &item, &p)) return;
+    if (!find_item(b, v.n_seqs, v.max_len, group, blockIdx.x, &seq, &item, &p)) return;
     const bool key = blockIdx.z == 0;
     const Rows &x = key ? k : val;
     const uint32_t head = blockIdx.y, sh = seq * v.n_heads + head;
@@ -268,8 +378,9 @@ template <int NC, int WAVES> __global__ void __launch_bounds__(256, WAVES) write
         return (uint64_t)(p.s.row + (uint32_t)((int64_t)pos - p.s.pos)) * x.ld_row + head * x.ld_head;
     };
     if (item) {
-        const uint32_t blk = p.b0 + item;
-        write_block<NC>(v, x, row_at(blk * kBlock), x.ld_row, sh, base, blk, 0, kBlock, -1, false, false, key, maxes, red, stage);
+        const uint32_t blk = p.b0 + 1 + (item - 1) * group;
+        const uint32_t count = min(group, p.end / kBlock - blk);
+        write_whole<NC>(v, x, row_at(blk * kBlock), base, blk, count, key, red, stage);
         return;
     }
     int32_t *at = v.tail_at + base * 4;
@@ -293,12 +404,12 @@ template <int NC, int WAVES> __global__ void __launch_bounds__(256, WAVES) write
         tag[slot] = (int32_t)p.b0;
         fill[slot] = (int32_t)hi;
     }
-    write_block<NC>(v, x, row_at(p.first), x.ld_row, sh, base, p.b0, lo, hi, slot, held, open, key, maxes, red, stage);
+    write_block<NC>(v, x, row_at(p.first), base, p.b0, lo, hi, slot, held, open, key, maxes, red[0], stage);
     if (p.bl > p.b0 && p.end % kBlock) {
         const int other = held ? 1 - slot : tag[0] <= tag[1] ? 0 : 1;
         tag[other] = (int32_t)p.bl;
         fill[other] = (int32_t)(p.end % kBlock);
-        write_block<NC>(v, x, row_at(p.bl * kBlock), x.ld_row, sh, base, p.bl, 0, p.end % kBlock, other, false, true, key, maxes, red,
+        write_block<NC>(v, x, row_at(p.bl * kBlock), base, p.bl, 0, p.end % kBlock, other, false, true, key, maxes, red[0],
                         stage);
     }
     if (threadIdx.x == 0) {
@@ -384,17 +495,18 @@ int launched()
 int launch_write(const View &v, const Batch &b, const Rows &k, const Rows &x, int n_cu, hipStream_t st)
 {
     if (b.n_rows == 0) return 0;
-    // items of a sequence of n rows: at most (n + 30) / 32 + 1, and one for one row
-    const uint64_t most = b.starts ? (uint64_t)b.n_rows / kBlock + 2ull * std::min(v.n_seqs, b.n_rows)
-                          : b.lens ? b.n_rows : b.n_rows / kBlock + 2u;
-    const dim3 grid((uint32_t)most, v.n_heads, 2);
-    // more workgroups than fit with the registers they would like (5 a compute
-    // unit): as many as there can be (us: 32 prompts of up to 2048 tokens 62.4
-    // against 73.1; 1001 tokens 9.1 against 8.5, one token 5.2 against 4.6)
-    const bool crowd = most * v.n_heads * 2 > 5ull * (uint32_t)(n_cu > 0 ? n_cu : 256);
-    if (v.dp > 128) hipLaunchKernelGGL((write_k<2, 1>), grid, dim3(256), 0, st, v, b, k, x);
-    else if (crowd) hipLaunchKernelGGL((write_k<1, 8>), grid, dim3(256), 0, st, v, b, k, x);
-    else hipLaunchKernelGGL((write_k<1, 1>), grid, dim3(256), 0, st, v, b, k, x);
+    const uint64_t seqs = b.starts ? std::min(v.n_seqs, b.n_rows) : 1u;
+    const bool one = b.lens && !b.starts;                     // one row, one item for each sequence
+    // one block a workgroup while all of them are there at once (5 a compute unit
+    // fit); else four, each block's rows loaded during the one before (us, 32
+    // prompts of up to 2048 tokens: 54 against 66, two 62, eight 56; with 6
+    // workgroups a compute unit 68)
+    const uint64_t room = 5ull * (uint32_t)(n_cu > 0 ? n_cu : 256);
+    const uint32_t group = !one && ((uint64_t)b.n_rows / kBlock + 2 * seqs) * v.n_heads * 2 > room ? 4u : 1u;
+    // items of a sequence of n rows: at most n / (32 group) + 2
+    const dim3 grid(one ? b.n_rows : (uint32_t)(b.n_rows / (kBlock * group) + 2 * seqs), v.n_heads, 2);
+    if (v.dp > 128) hipLaunchKernelGGL((write_k<2>), grid, dim3(256), 0, st, v, b, k, x, group);
+    else hipLaunchKernelGGL((write_k<1>), grid, dim3(256), 0, st, v, b, k, x, group);
     return launched();
 }
 

@@ -102,6 +102,25 @@ def test_prompt_and_steps(rinf, ctx, hd, dtype):
     cache.free()
 
 
+@pytest.mark.parametrize("hd,heads,dtype", [(16, 40, "f32"), (5, 48, "f16"), (128, 33, "f16"), (200, 33, "f32"), (64, 64, "f16")])
+def test_long_prompts(rinf, ctx, hd, heads, dtype):
+    """More blocks than workgroups fit, so that one takes several: prompts of all
+    remainders, then more rows from inside a block on; a NaN and zeros in the middle."""
+    rng = np.random.default_rng(hd)
+    first, then = [700, 129, 0, 384, 33], [1, 450, 320, 0, 95]
+    total = [a + b for a, b in zip(first, then)]
+    cache = ctx.kv8(len(total), heads, hd, max(total))
+    hk = [rows(rng, n, heads, hd, dtype) for n in total]
+    hv = [rows(rng, n, heads, hd, dtype) for n in total]
+    hk[0][333, 1, hd - 1], hv[1][200, 2, 0] = np.nan, np.inf
+    hk[0][96:160, 3], hv[2][64:96, 4] = 0, 0
+    for call in range(2):
+        k, v = ([x[:a] if call == 0 else x[a:] for x, a in zip(h, first)] for h in (hk, hv))
+        write(ctx, cache, k, v, first if call == 0 else total)
+        check(ctx, cache, *([x[:a] for x, a in zip(h, first)] if call == 0 else h for h in (hk, hv)))
+    cache.free()
+
+
 @pytest.mark.parametrize("seed", range(4))
 def test_any_calls_give_one_cache(rinf, ctx, seed):
     """Calls of 0 to 100 rows a sequence, in any ragged mix."""
