@@ -127,7 +127,7 @@ int qg_model_resident_bytes(qg_model *m, size_t *weights, size_t *file_bytes, si
 
 /* No counterpart in the reference: keep the KV caches in 8 bits (enable != 0;
  * qg_kv8 of qgops.h, one per layer) instead of f32, in about a quarter of the
- * memory: the decode step and both prefills then quantise their keys and values
+ * memory (and 17 to 80 MB of workspace, once a model): the decode step and both prefills then quantise their keys and values
  * as they are written and attend over the codes (any head_dim up to 256, any
  * length; QG_ERR_SHAPE beyond).  Tokens of one prefill chunk see the caches as
  * they are when the chunk is written, so a block's scale may come from a later

@@ -126,8 +126,20 @@ __device__ __forceinline__ void store1(const Rows &r, uint64_t at, float v)
     else ((float *)r.p)[at] = v;
 }
 
+// A decode step's projections of one token, on the device: q [kv head][n_rep][hd]
+// is rotated in place, k and v [kv head][hd] are left as they are.  pos: of the
+// rotation (rows of the tables, hd / 2 each); slot: in the cache; *len becomes
+// slot + 1.
+struct Append {
+    float *q;
+    const float *k, *v, *bq, *bk, *bv, *cos_t, *sin_t;
+    const uint32_t *pos, *slot;
+    uint32_t *len, n_rep;
+};
+
 // Launchers; 0, or -1 for a failed launch (hipGetLastError holds it).
 int launch_write(const View &c, const Batch &b, const Rows &k, const Rows &v, int n_cu, hipStream_t st);
+int launch_append(const View &c, const Append &a, hipStream_t st);
 int launch_read(const View &c, uint32_t seq, uint32_t n_seqs, uint32_t pos, uint32_t n, const Rows *k, const Rows *v,
                 hipStream_t st);
 int launch_attention(const View &c, const Batch &b, uint32_t n_heads, const Rows &q, float scale, uint32_t window,

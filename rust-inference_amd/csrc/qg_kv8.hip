@@ -157,19 +157,19 @@ __device__ __forceinline__ void put_values(const uint8_t *stage, uint8_t *codes,
     }
 }
 
-// Block `b`'s positions lo .. hi (of 32) from the rows, those before lo from
-// what the cache holds.  One workgroup of 256: thread (t, c): position t =
-// tid / 8, elements 16 (c + 8 i) .. + 16.
-template <int NC>
-__device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint64_t base, uint32_t b, uint32_t lo,
-                            uint32_t hi, int slot, bool held, bool open, bool key, uint32_t *maxes, uint32_t *red,
-                            uint8_t *stage)
+// Block `b`'s positions lo .. hi (of 32) from the rows (load(r, d, y): elements d
+// .. d + 16 of the r-th one, zero from head_dim on), those before lo from what
+// the cache holds.  One workgroup of 256: thread (t, c): position t = tid / 8,
+// elements 16 (c + 8 i) .. + 16.
+template <int NC, class Load>
+__device__ void write_block(const View &v, Load load, uint64_t base, uint32_t b, uint32_t lo, uint32_t hi, uint32_t slot,
+                            bool held, bool open, bool key, uint32_t *maxes, uint32_t *red, uint8_t *stage)
 {
     const uint32_t tid = threadIdx.x, t = tid >> 3, c = tid & 7u, dp = v.dp;
     uint8_t *codes = v.codes + (base * v.n_blocks + b) * kBlock * dp;
     float *scale = v.scale + base * v.n_blocks + b;
-    float *tail = v.tail + (base * 2 + (uint32_t)(slot < 0 ? 0 : slot)) * kBlock * dp + t * dp;
-    uint32_t *tail_max = v.tail_max + (base * 2 + (uint32_t)(slot < 0 ? 0 : slot)) * kBlock;
+    float *tail = v.tail + (base * 2 + slot) * kBlock * dp + t * dp;
+    uint32_t *tail_max = v.tail_max + (base * 2 + slot) * kBlock;
     float val[NC][16];
     const bool fresh = t >= lo && t < hi, old = t < lo;
     const float s_old = lo ? *scale : 0.f;
@@ -180,7 +180,7 @@ __device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint6
         const uint32_t d = 16u * (c + 8u * i);
         if (d >= dp) break;
         if (fresh) {
-            load16(x, row_at + (uint64_t)(t - lo) * x.ld_row, d, v.hd, val[i]);
+            load(t - lo, d, val[i]);
         } else {
 #pragma unroll
             for (int j = 0; j < 16; j++) val[i][j] = 0.f;
@@ -250,6 +250,44 @@ __device__ void write_block(const View &v, const Rows &x, uint64_t row_at, uint6
     if (tid == 0) *scale = s;
     if (open && tid < hi && (tid >= lo || !held)) tail_max[tid] = maxes[tid];
     __syncthreads();
+}
+
+// The slots of f32 rows of a head: their blocks (-1: none) and the positions held
+// of each; the one that block b0 takes, and whether it holds what lies before the
+// call's rows lo .. hi of that block.
+struct Tail {
+    int32_t tag[2], fill[2];
+    uint32_t slot;
+    bool held;
+};
+
+__device__ __forceinline__ Tail take_tail(const int32_t *at, uint32_t b0, uint32_t lo, uint32_t hi)
+{
+    Tail a{{at[0], at[1]}, {at[2], at[3]}, 0, false};
+    __syncthreads();                                          // read by all before put_tail
+    // what is held of this block from lo on, or of later ones, is written anew
+    for (int i = 0; i < 2; i++) {
+        if (a.tag[i] == (int32_t)b0) a.fill[i] = min(a.fill[i], (int32_t)lo);
+        if (a.tag[i] > (int32_t)b0 || (a.tag[i] == (int32_t)b0 && a.fill[i] == 0)) a.tag[i] = -1;
+    }
+    const int slot = a.tag[0] == (int32_t)b0 ? 0 : a.tag[1] == (int32_t)b0 ? 1 : -1;
+    a.held = slot >= 0 && a.fill[slot] >= (int32_t)lo;
+    if (slot >= 0 && !a.held) a.tag[slot] = -1;
+    a.slot = a.held ? (uint32_t)slot : a.tag[0] <= a.tag[1] ? 0u : 1u;       // else the older one gives way
+    if (hi < kBlock) {
+        a.tag[a.slot] = (int32_t)b0;
+        a.fill[a.slot] = (int32_t)hi;
+    }
+    return a;
+}
+
+__device__ __forceinline__ void put_tail(int32_t *at, const Tail &a)
+{
+    if (threadIdx.x) return;
+    at[0] = a.tag[0];
+    at[1] = a.tag[1];
+    at[2] = a.fill[0];
+    at[3] = a.fill[1];
 }
 
 // A thread's 16 elements of a row as they lie in memory: f16 in two words, else
@@ -383,41 +421,61 @@ __global__ void __launch_bounds__(256, NC == 1 ? 5 : 2) write_k(View v, Batch b,
         write_whole<NC>(v, x, row_at(blk * kBlock), base, blk, count, key, red, stage);
         return;
     }
-    int32_t *at = v.tail_at + base * 4;
-    int32_t tag[2] = {at[0], at[1]}, fill[2] = {at[2], at[3]};
-    __syncthreads();                                          // read by all before thread 0 writes
     const uint32_t lo = p.first % kBlock, hi = p.bl == p.b0 ? p.end - p.b0 * kBlock : kBlock;
-    // what is held of this block from lo on, or of later ones, is written anew
-    for (int i = 0; i < 2; i++) {
-        if (tag[i] == (int32_t)p.b0) fill[i] = min(fill[i], (int32_t)lo);
-        if (tag[i] > (int32_t)p.b0 || (tag[i] == (int32_t)p.b0 && fill[i] == 0)) tag[i] = -1;
-    }
-    int slot = tag[0] == (int32_t)p.b0 ? 0 : tag[1] == (int32_t)p.b0 ? 1 : -1;
-    bool held = slot >= 0 && fill[slot] >= (int32_t)lo;
-    if (slot >= 0 && !held) { tag[slot] = -1; }
-    const bool open = hi < kBlock;
-    if (slot < 0 || !held) {
-        slot = tag[0] <= tag[1] ? 0 : 1;                      // the older one gives way
-        held = false;
-    }
-    if (open) {
-        tag[slot] = (int32_t)p.b0;
-        fill[slot] = (int32_t)hi;
-    }
-    write_block<NC>(v, x, row_at(p.first), base, p.b0, lo, hi, slot, held, open, key, maxes, red[0], stage);
+    Tail tail = take_tail(v.tail_at + base * 4, p.b0, lo, hi);
+    auto rows_from = [&](uint32_t pos) {
+        const uint64_t first = row_at(pos);
+        return [&, first](uint32_t r, uint32_t d, float *y) { load16(x, first + (uint64_t)r * x.ld_row, d, v.hd, y); };
+    };
+    write_block<NC>(v, rows_from(p.first), base, p.b0, lo, hi, tail.slot, tail.held, hi < kBlock, key, maxes, red[0], stage);
     if (p.bl > p.b0 && p.end % kBlock) {
-        const int other = held ? 1 - slot : tag[0] <= tag[1] ? 0 : 1;
-        tag[other] = (int32_t)p.bl;
-        fill[other] = (int32_t)(p.end % kBlock);
-        write_block<NC>(v, x, row_at(p.bl * kBlock), base, p.bl, 0, p.end % kBlock, other, false, true, key, maxes, red[0],
+        const uint32_t other = tail.held ? 1 - tail.slot : tail.tag[0] <= tail.tag[1] ? 0 : 1;
+        tail.tag[other] = (int32_t)p.bl;
+        tail.fill[other] = (int32_t)(p.end % kBlock);
+        write_block<NC>(v, rows_from(p.bl * kBlock), base, p.bl, 0, p.end % kBlock, other, false, true, key, maxes, red[0],
                         stage);
     }
-    if (threadIdx.x == 0) {
-        at[0] = tag[0];
-        at[1] = tag[1];
-        at[2] = fill[0];
-        at[3] = fill[1];
+    put_tail(v.tail_at + base * 4, tail);
+}
+
+// A decode step's projections of one token (Append): q and k with their biases
+// rotated, v with its own, k and v written as the token's place of a cache of one
+// sequence.  Grid: (1, kv heads, keys / values / the kv head's query heads).
+// One launch for what was two (qkv rotation, write_k), each a few dependent loads.
+template <int NC> __global__ void __launch_bounds__(256) append_k(View v, Append a)
+{
+    __shared__ uint32_t maxes[kBlock], red[4];
+    __shared__ __attribute__((aligned(16))) uint8_t stage[kBlock * (128 * NC + 16)];
+    const uint32_t pos = *a.pos, at = *a.slot, head = blockIdx.y, hd = v.hd;
+    const float *cs = a.cos_t + (size_t)pos * (hd / 2), *sn = a.sin_t + (size_t)pos * (hd / 2);
+    if (blockIdx.z == 2) {
+        for (uint32_t i = 2 * threadIdx.x; i < a.n_rep * hd; i += 512) {
+            const uint32_t e = head * a.n_rep * hd + i, j = i % hd / 2;
+            const float x0 = a.q[e] + a.bq[e], x1 = a.q[e + 1] + a.bq[e + 1];
+            a.q[e] = x0 * cs[j] - x1 * sn[j];
+            a.q[e + 1] = x0 * sn[j] + x1 * cs[j];
+        }
+        if (head == 0 && threadIdx.x == 0) *a.len = at + 1;
+        return;
     }
+    if (at >= v.max_len) return;
+    const bool key = blockIdx.z == 0;
+    const float *x = (key ? a.k : a.v) + head * hd, *b = (key ? a.bk : a.bv) + head * hd;
+    const uint64_t base = (uint64_t)blockIdx.z * v.n_heads + head;
+    const uint32_t lo = at % kBlock, blk = at / kBlock;
+    const Tail tail = take_tail(v.tail_at + base * 4, blk, lo, lo + 1);
+    auto row = [&](uint32_t, uint32_t d, float *y) {
+#pragma unroll
+        for (uint32_t j = 0; j < 16; j += 2) {
+            const bool in = d + j < hd;                       // hd is even
+            const float x0 = in ? x[d + j] + b[d + j] : 0.f, x1 = in ? x[d + j + 1] + b[d + j + 1] : 0.f;
+            const float c = in && key ? cs[(d + j) / 2] : 1.f, s = in && key ? sn[(d + j) / 2] : 0.f;
+            y[j] = key ? x0 * c - x1 * s : x0;
+            y[j + 1] = key ? x0 * s + x1 * c : x1;
+        }
+    };
+    write_block<NC>(v, row, base, blk, lo, lo + 1, tail.slot, tail.held, lo + 1 < kBlock, key, maxes, red, stage);
+    put_tail(v.tail_at + base * 4, tail);
 }
 
 // Grid: (blocks, heads * keys / values, sequences); 256 threads.  A thread takes 16
@@ -507,6 +565,14 @@ int launch_write(const View &v, const Batch &b, const Rows &k, const Rows &x, in
     const dim3 grid(one ? b.n_rows : (uint32_t)(b.n_rows / (kBlock * group) + 2 * seqs), v.n_heads, 2);
     if (v.dp > 128) hipLaunchKernelGGL((write_k<2>), grid, dim3(256), 0, st, v, b, k, x, group);
     else hipLaunchKernelGGL((write_k<1>), grid, dim3(256), 0, st, v, b, k, x, group);
+    return launched();
+}
+
+int launch_append(const View &v, const Append &a, hipStream_t st)
+{
+    const dim3 grid(1, v.n_heads, 3);
+    if (v.dp > 128) hipLaunchKernelGGL((append_k<2>), grid, dim3(256), 0, st, v, a);
+    else hipLaunchKernelGGL((append_k<1>), grid, dim3(256), 0, st, v, a);
     return launched();
 }
 

@@ -24,8 +24,9 @@
 //                    rescaled)
 //   qkv_post_k       the bias add, RoPE and KV append alone, and
 //   attention_k      attention in one workgroup per head (other head_dim)
-//   qkv_rope_k       the bias add and RoPE alone, before the 8-bit caches' write and
-//                    attention (qg_kv8.hip, qg_kv8_attention.hip; qg_model_use_kv8)
+//   qg8::append_k    the bias add, RoPE and the write into an 8-bit cache, before
+//                    the attention over it (qg_kv8.hip, qg_kv8_attention.hip;
+//                    qg_model_use_kv8)
 //   SiLU * up        mlp.rs:31-43, silu as math.rs:137-146, in the epilogue
 //                    of the [gate; up] GEMV (gate and up rows paired), else
 //                    inside the down GEMV's prologue or a separate kernel
@@ -166,35 +167,6 @@ __global__ void __launch_bounds__(256) qkv_post_k(float *__restrict__ q, const f
         kr[i0 + 1] = x0 * s + x1 * c;
         vr[i0] = v[i0] + bv[i0];
         vr[i0 + 1] = v[i0 + 1] + bv[i0 + 1];
-    }
-}
-
-// The same without a cache to append to (8-bit caches): k and v in place, and
-// the number of positions with this one.
-__global__ void __launch_bounds__(256) qkv_rope_k(float *__restrict__ q, float *__restrict__ k, float *__restrict__ v,
-                                                  const float *__restrict__ bq, const float *__restrict__ bk,
-                                                  const float *__restrict__ bv, const float *__restrict__ cos_t,
-                                                  const float *__restrict__ sin_t, uint32_t q_dim, uint32_t kv_dim,
-                                                  uint32_t hd, const Step *__restrict__ st, uint32_t *__restrict__ len)
-{
-    const uint32_t t = blockIdx.x * blockDim.x + threadIdx.x, half = hd / 2;
-    const uint32_t pos = st->pos, i0 = 2 * t;
-    if (t == 0) *len = st->slot + 1;
-    if (i0 < q_dim) {
-        const uint32_t j = (i0 % hd) / 2;
-        const float c = cos_t[(size_t)pos * half + j], s = sin_t[(size_t)pos * half + j];
-        const float x0 = q[i0] + bq[i0], x1 = q[i0 + 1] + bq[i0 + 1];
-        q[i0] = x0 * c - x1 * s;
-        q[i0 + 1] = x0 * s + x1 * c;
-    }
-    if (i0 < kv_dim) {
-        const uint32_t j = (i0 % hd) / 2;
-        const float c = cos_t[(size_t)pos * half + j], s = sin_t[(size_t)pos * half + j];
-        const float x0 = k[i0] + bk[i0], x1 = k[i0 + 1] + bk[i0 + 1];
-        k[i0] = x0 * c - x1 * s;
-        k[i0 + 1] = x0 * s + x1 * c;
-        v[i0] += bv[i0];
-        v[i0 + 1] += bv[i0 + 1];
     }
 }
 
@@ -1378,17 +1350,25 @@ qg8::Rows kv8_rows(const qg_model *m, const float *p, size_t ld)
     return r;
 }
 
-// Caches the rows' k and v in layer l and attends: the positions end at
-// b.len0 or, for the decode step's one row, at *kv8_len.
-int kv8_attention(qg_model *m, uint32_t l, const qg8::Batch &b, const float *q, size_t ldq, const float *k, size_t ldk,
-                  const float *v, size_t ldv, float *out)
+// Attends over layer l's cache; the positions end at b.len0 or, for the decode
+// step's one row, at *kv8_len.
+int kv8_attend(qg_model *m, uint32_t l, const qg8::Batch &b, const float *q, size_t ldq, float *out)
 {
-    const qg8::View &c = m->kv8[l]->v;
-    if (qg8::launch_write(c, b, kv8_rows(m, k, ldk), kv8_rows(m, v, ldv), m->ctx->n_cu, m->ctx->stream) ||
-        qg8::launch_attention(c, b, m->cfg.n_heads, kv8_rows(m, q, ldq), 1.0f / sqrtf((float)m->hd), 0,
+    if (qg8::launch_attention(m->kv8[l]->v, b, m->cfg.n_heads, kv8_rows(m, q, ldq), 1.0f / sqrtf((float)m->hd), 0,
                               kv8_rows(m, out, m->q_dim), m->kv8_work, m->ctx->n_cu, m->ctx->stream))
         return mfail(m, QG_ERR_HIP, "attention over the 8-bit cache", hipGetLastError());
     return QG_OK;
+}
+
+// The same for a chunk of ntok tokens from position s0 on, whose k and v are in
+// kv8_k and kv8_v and are cached first.
+int kv8_chunk(qg_model *m, uint32_t l, uint32_t s0, uint32_t ntok, const float *q, size_t ldq, float *out)
+{
+    const qg8::Batch b{nullptr, nullptr, ntok, s0 + ntok};
+    if (qg8::launch_write(m->kv8[l]->v, b, kv8_rows(m, m->kv8_k, m->kv_dim), kv8_rows(m, m->kv8_v, m->kv_dim),
+                          m->ctx->n_cu, m->ctx->stream))
+        return mfail(m, QG_ERR_HIP, "8-bit cache", hipGetLastError());
+    return kv8_attend(m, l, b, q, ldq, out);
 }
 
 int launched(qg_model *m, const char *what)
@@ -1455,12 +1435,16 @@ int enqueue_forward(qg_model *m)
         }
         float *kc = m->kc + l * kv_layer, *vc = m->vc + l * kv_layer;
         if (!m->kv8.empty()) {
-            hipLaunchKernelGGL(qgm::qkv_rope_k, dim3((pairs + 255) / 256), dim3(256), 0, st, m->q, m->k, m->v,
-                               m->vec[QG_V_BQ][l], m->vec[QG_V_BK][l], m->vec[QG_V_BV][l], m->cos_t, m->sin_t, m->q_dim,
-                               m->kv_dim, m->hd, m->d_step, m->kv8_len);
-            if ((rc = kv8_attention(m, l, qg8::Batch{nullptr, m->kv8_len, 1, 0}, m->q, m->q_dim, m->k, m->kv_dim, m->v,
-                                    m->kv_dim, m->ao)))
-                return rc;
+            qg8::Append ap{};
+            ap.q = m->q; ap.k = m->k; ap.v = m->v;
+            ap.bq = m->vec[QG_V_BQ][l]; ap.bk = m->vec[QG_V_BK][l]; ap.bv = m->vec[QG_V_BV][l];
+            ap.cos_t = m->cos_t; ap.sin_t = m->sin_t;
+            ap.pos = &m->d_step->pos; ap.slot = &m->d_step->slot;
+            ap.len = m->kv8_len;
+            ap.n_rep = m->n_rep;
+            if (qg8::launch_append(m->kv8[l]->v, ap, st))
+                return mfail(m, QG_ERR_HIP, "8-bit cache", hipGetLastError());
+            if ((rc = kv8_attend(m, l, qg8::Batch{nullptr, m->kv8_len, 1, 0}, m->q, m->q_dim, m->ao))) return rc;
         } else if (m->att_grp) {
             qgm::AttnArgs aa{};
             aa.q = m->q; aa.k = m->k; aa.v = m->v;
@@ -1830,9 +1814,7 @@ int pf_chunk(qg_model *m, const uint32_t *d_tok, uint32_t ntok, uint32_t s0, boo
             (!kv8 && qg::launch_pf_attention(m->pf_qkv, ldq, kc, vc, m->pf_ao, c.n_heads, m->hd, m->kv_dim, m->n_rep,
                                              scale, s0, ntok, sti)))
             return mfail(m, QG_ERR_HIP, "prefill attention", hipGetLastError());
-        if (kv8 && (rc = kv8_attention(m, l, qg8::Batch{nullptr, nullptr, ntok, s0 + ntok}, m->pf_qkv, ldq, kc, m->kv_dim,
-                                       vc, m->kv_dim, m->pf_ao)))
-            return rc;
+        if (kv8 && (rc = kv8_chunk(m, l, s0, ntok, m->pf_qkv, ldq, m->pf_ao))) return rc;
         const qg::PfMat wo = pf_mat(m->w[QG_M_WO - 2][l], m->pf_ao2);
         if ((rc = pf_planes(m, m->pf_ao, 1, nullptr, 0, nullptr, nullptr, m->q_dim, m->q_dim, 0, false, ntok)) ||
             (rc = pf_gemm(m, &wo, 1, m->q_dim, ntok, E, m->pf_s_o)))
@@ -2003,9 +1985,7 @@ int wide_chunk(qg_model *m, const uint32_t *d_tok, uint32_t ntok, uint32_t s0, b
             (!kv8 && qg::launch_wide_attention(m->wd_qkv, ldq, kc, vc, m->wd_ao, c.n_heads, m->hd, m->kv_dim, m->n_rep,
                                                scale, s0, ntok, sti)))
             return mfail(m, QG_ERR_HIP, "prefill attention", hipGetLastError());
-        if (kv8 && (rc = kv8_attention(m, l, qg8::Batch{nullptr, nullptr, ntok, s0 + ntok}, m->wd_qkv, ldq, kc, m->kv_dim,
-                                       vc, m->kv_dim, m->wd_ao)))
-            return rc;
+        if (kv8 && (rc = kv8_chunk(m, l, s0, ntok, m->wd_qkv, ldq, m->wd_ao))) return rc;
         const qg::PfMat wo = pf_mat(m->w[QG_M_WO - 2][l], m->wd_ao2);
         if ((rc = wide_planes(m, m->wd_ao, 1, nullptr, 0, 0, nullptr, nullptr, m->q_dim, m->q_dim, 0, ntok)) ||
             (rc = wide_gemm(m, &wo, 1, m->q_dim, ntok, E, sp.o, T * E)) ||
