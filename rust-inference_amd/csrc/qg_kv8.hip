@@ -157,39 +157,90 @@ __device__ __forceinline__ void put_values(const uint8_t *stage, uint8_t *codes,
     }
 }
 
-// Block `b`'s positions lo .. hi (of 32) from the rows (load(r, d, y): elements d
-// .. d + 16 of the r-th one, zero from head_dim on), those before lo from what
-// the cache holds.  One workgroup of 256: thread (t, c): position t = tid / 8,
-// elements 16 (c + 8 i) .. + 16.
-template <int NC, class Load>
-__device__ void write_block(const View &v, Load load, uint64_t base, uint32_t b, uint32_t lo, uint32_t hi, uint32_t slot,
-                            bool held, bool open, bool key, uint32_t *maxes, uint32_t *red, uint8_t *stage)
+// The slots of f32 rows of a head: their blocks (-1: none) and the positions held
+// of each; the one that block b0 takes, and whether it holds what lies before the
+// call's rows lo .. hi of that block.
+struct Tail {
+    int32_t tag0, tag1, fill0, fill1;
+    uint32_t slot;
+    bool held;
+};
+
+// The slot holds positions 0 .. n of block b.
+__device__ __forceinline__ void hold(Tail &a, uint32_t b, uint32_t n)
+{
+    a.tag0 = a.slot ? a.tag0 : (int32_t)b;
+    a.fill0 = a.slot ? a.fill0 : (int32_t)n;
+    a.tag1 = a.slot ? (int32_t)b : a.tag1;
+    a.fill1 = a.slot ? (int32_t)n : a.fill1;
+}
+
+__device__ __forceinline__ Tail take_tail(int4 at, uint32_t b0, uint32_t lo, uint32_t hi)
+{
+    const int32_t b = (int32_t)b0, n = (int32_t)lo;
+    Tail a;
+    // what is held of this block from lo on, or of later ones, is written anew
+    a.fill0 = at.x == b ? min(at.z, n) : at.z;
+    a.fill1 = at.y == b ? min(at.w, n) : at.w;
+    a.tag0 = at.x > b || (at.x == b && a.fill0 < n) || (at.x == b && n == 0) ? -1 : at.x;
+    a.tag1 = at.y > b || (at.y == b && a.fill1 < n) || (at.y == b && n == 0) ? -1 : at.y;
+    a.held = a.tag0 == b || a.tag1 == b;
+    a.slot = a.held ? (a.tag0 == b ? 0u : 1u) : (a.tag0 <= a.tag1 ? 0u : 1u);      // else the older one gives way
+    if (hi < kBlock) hold(a, b0, hi);
+    return a;
+}
+
+__device__ __forceinline__ void put_tail(int32_t *at, const Tail &a)
+{
+    if (threadIdx.x == 0) *(int4 *)at = make_int4(a.tag0, a.tag1, a.fill0, a.fill1);
+}
+
+// Block `b`'s positions lo .. hi (of 32) from the rows (load(r, i, d, y): elements
+// d = 16 (c + 8 i) .. + 16 of the r-th one, zero from head_dim on), those before
+// lo from what the cache holds.  One workgroup of 256: thread (t, c): position t =
+// tid / 8, elements 16 (c + 8 i) .. + 16.  FIRST: the call's first block, which
+// takes its slot; else a new one (lo = 0) in the slot of `tail`.  All that may be
+// needed of the head is asked for before any of it is looked at.
+template <int NC, bool FIRST, class Load>
+__device__ void write_block(const View &v, Load load, uint64_t base, uint32_t b, uint32_t lo, uint32_t hi, Tail &tail,
+                            bool key, uint32_t *maxes, uint32_t *red, uint8_t *stage)
 {
     const uint32_t tid = threadIdx.x, t = tid >> 3, c = tid & 7u, dp = v.dp;
     uint8_t *codes = v.codes + (base * v.n_blocks + b) * kBlock * dp;
     float *scale = v.scale + base * v.n_blocks + b;
-    float *tail = v.tail + (base * 2 + slot) * kBlock * dp + t * dp;
-    uint32_t *tail_max = v.tail_max + (base * 2 + slot) * kBlock;
-    float val[NC][16];
-    const bool fresh = t >= lo && t < hi, old = t < lo;
-    const float s_old = lo ? *scale : 0.f;
-    uint32_t m;
-    float top = 0.f;
+    uint32_t *maxes_of = v.tail_max + base * 2 * kBlock;
+    const bool fresh = t >= lo && t < hi, old = t < lo, open = hi < kBlock;
+    float s_old = 0.f;
+    uint32_t m0 = 0, m1 = 0;
+    int4 at;
+    if (FIRST) {
+        at = *(const int4 *)(v.tail_at + base * 4);
+        s_old = *scale;
+        m0 = maxes_of[t];
+        m1 = maxes_of[kBlock + t];
+    }
+    float val[NC][16], top = 0.f;
 #pragma unroll
     for (int i = 0; i < NC; i++) {
         const uint32_t d = 16u * (c + 8u * i);
         if (d >= dp) break;
-        if (fresh) {
-            load(t - lo, d, val[i]);
-        } else {
 #pragma unroll
-            for (int j = 0; j < 16; j++) val[i][j] = 0.f;
-            if (old && !held)          // a block reopened from its codes
-                for (uint32_t j = 0; j < 16; j++) {
-                    const int q = (int)codes[key ? key_at(t, d + j, dp) : value_at(t, d + j)] - kZero;
-                    val[i][j] = (float)q * s_old;
-                }
-        }
+        for (int j = 0; j < 16; j++) val[i][j] = 0.f;
+        if (fresh) load(t - lo, i, d, val[i]);
+    }
+    if (FIRST) tail = take_tail(at, b, lo, hi);
+    const bool held = FIRST && tail.held;
+    float *rows = v.tail + (base * 2 + tail.slot) * kBlock * dp + t * dp;
+    uint32_t m;
+#pragma unroll
+    for (int i = 0; i < NC; i++) {
+        const uint32_t d = 16u * (c + 8u * i);
+        if (d >= dp) break;
+        if (old && !held)              // a block reopened from its codes
+            for (uint32_t j = 0; j < 16; j++) {
+                const int q = (int)codes[key ? key_at(t, d + j, dp) : value_at(t, d + j)] - kZero;
+                val[i][j] = (float)q * s_old;
+            }
 #pragma unroll
         for (int j = 0; j < 16; j++) top = __builtin_elementwise_maximum(top, fabsf(val[i][j]));    // NaN if any is
     }
@@ -198,7 +249,7 @@ __device__ void write_block(const View &v, Load load, uint64_t base, uint32_t b,
     m = max(m, (uint32_t)__shfl_xor((int)m, 1, 64));
     m = max(m, (uint32_t)__shfl_xor((int)m, 2, 64));
     m = max(m, (uint32_t)__shfl_xor((int)m, 4, 64));
-    if (old && held) m = tail_max[t];
+    if (old && held) m = tail.slot ? m1 : m0;
     if (c == 0) maxes[t] = m;
     m = wave_max_u(m);
     if ((tid & 63u) == 0) red[tid >> 6] = m;
@@ -215,7 +266,7 @@ __device__ void write_block(const View &v, Load load, uint64_t base, uint32_t b,
             if (d >= dp) break;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float4 a = *(const float4 *)(tail + d + 4 * j);
+                const float4 a = *(const float4 *)(rows + d + 4 * j);
                 val[i][4 * j] = a.x; val[i][4 * j + 1] = a.y; val[i][4 * j + 2] = a.z; val[i][4 * j + 3] = a.w;
             }
         }
@@ -240,7 +291,7 @@ __device__ void write_block(const View &v, Load load, uint64_t base, uint32_t b,
         if (open && (fresh || (old && !held)))
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                *(float4 *)(tail + d + 4 * j) = make_float4(val[i][4 * j], val[i][4 * j + 1], val[i][4 * j + 2],
+                *(float4 *)(rows + d + 4 * j) = make_float4(val[i][4 * j], val[i][4 * j + 1], val[i][4 * j + 2],
                                                             val[i][4 * j + 3]);
     }
     if (!key && whole) {
@@ -248,46 +299,8 @@ __device__ void write_block(const View &v, Load load, uint64_t base, uint32_t b,
         put_values(stage, codes, dp);
     }
     if (tid == 0) *scale = s;
-    if (open && tid < hi && (tid >= lo || !held)) tail_max[tid] = maxes[tid];
+    if (open && tid < hi && (tid >= lo || !held)) maxes_of[tail.slot * kBlock + tid] = maxes[tid];
     __syncthreads();
-}
-
-// The slots of f32 rows of a head: their blocks (-1: none) and the positions held
-// of each; the one that block b0 takes, and whether it holds what lies before the
-// call's rows lo .. hi of that block.
-struct Tail {
-    int32_t tag[2], fill[2];
-    uint32_t slot;
-    bool held;
-};
-
-__device__ __forceinline__ Tail take_tail(const int32_t *at, uint32_t b0, uint32_t lo, uint32_t hi)
-{
-    Tail a{{at[0], at[1]}, {at[2], at[3]}, 0, false};
-    __syncthreads();                                          // read by all before put_tail
-    // what is held of this block from lo on, or of later ones, is written anew
-    for (int i = 0; i < 2; i++) {
-        if (a.tag[i] == (int32_t)b0) a.fill[i] = min(a.fill[i], (int32_t)lo);
-        if (a.tag[i] > (int32_t)b0 || (a.tag[i] == (int32_t)b0 && a.fill[i] == 0)) a.tag[i] = -1;
-    }
-    const int slot = a.tag[0] == (int32_t)b0 ? 0 : a.tag[1] == (int32_t)b0 ? 1 : -1;
-    a.held = slot >= 0 && a.fill[slot] >= (int32_t)lo;
-    if (slot >= 0 && !a.held) a.tag[slot] = -1;
-    a.slot = a.held ? (uint32_t)slot : a.tag[0] <= a.tag[1] ? 0u : 1u;       // else the older one gives way
-    if (hi < kBlock) {
-        a.tag[a.slot] = (int32_t)b0;
-        a.fill[a.slot] = (int32_t)hi;
-    }
-    return a;
-}
-
-__device__ __forceinline__ void put_tail(int32_t *at, const Tail &a)
-{
-    if (threadIdx.x) return;
-    at[0] = a.tag[0];
-    at[1] = a.tag[1];
-    at[2] = a.fill[0];
-    at[3] = a.fill[1];
 }
 
 // A thread's 16 elements of a row as they lie in memory: f16 in two words, else
@@ -422,18 +435,16 @@ __global__ void __launch_bounds__(256, NC == 1 ? 5 : 2) write_k(View v, Batch b,
         return;
     }
     const uint32_t lo = p.first % kBlock, hi = p.bl == p.b0 ? p.end - p.b0 * kBlock : kBlock;
-    Tail tail = take_tail(v.tail_at + base * 4, p.b0, lo, hi);
+    Tail tail;
     auto rows_from = [&](uint32_t pos) {
         const uint64_t first = row_at(pos);
-        return [&, first](uint32_t r, uint32_t d, float *y) { load16(x, first + (uint64_t)r * x.ld_row, d, v.hd, y); };
+        return [&, first](uint32_t r, int, uint32_t d, float *y) { load16(x, first + (uint64_t)r * x.ld_row, d, v.hd, y); };
     };
-    write_block<NC>(v, rows_from(p.first), base, p.b0, lo, hi, tail.slot, tail.held, hi < kBlock, key, maxes, red[0], stage);
+    write_block<NC, true>(v, rows_from(p.first), base, p.b0, lo, hi, tail, key, maxes, red[0], stage);
     if (p.bl > p.b0 && p.end % kBlock) {
-        const uint32_t other = tail.held ? 1 - tail.slot : tail.tag[0] <= tail.tag[1] ? 0 : 1;
-        tail.tag[other] = (int32_t)p.bl;
-        tail.fill[other] = (int32_t)(p.end % kBlock);
-        write_block<NC>(v, rows_from(p.bl * kBlock), base, p.bl, 0, p.end % kBlock, other, false, true, key, maxes, red[0],
-                        stage);
+        tail.slot = tail.held ? 1 - tail.slot : tail.tag0 <= tail.tag1 ? 0 : 1;
+        hold(tail, p.bl, p.end % kBlock);
+        write_block<NC, false>(v, rows_from(p.bl * kBlock), base, p.bl, 0, p.end % kBlock, tail, key, maxes, red[0], stage);
     }
     put_tail(v.tail_at + base * 4, tail);
 }
@@ -446,7 +457,18 @@ template <int NC> __global__ void __launch_bounds__(256) append_k(View v, Append
 {
     __shared__ uint32_t maxes[kBlock], red[4];
     __shared__ __attribute__((aligned(16))) uint8_t stage[kBlock * (128 * NC + 16)];
-    const uint32_t pos = *a.pos, at = *a.slot, head = blockIdx.y, hd = v.hd;
+    const uint32_t head = blockIdx.y, hd = v.hd;
+    const bool key = blockIdx.z == 0;
+    const float *x = (key ? a.k : a.v) + head * hd, *b = (key ? a.bk : a.bv) + head * hd;
+    float own[NC][16];                                        // asked for before the position is known
+    if (blockIdx.z < 2)
+#pragma unroll
+        for (int i = 0; i < NC; i++) {
+            const uint32_t d = 16u * ((threadIdx.x & 7u) + 8u * i);
+#pragma unroll
+            for (uint32_t j = 0; j < 16; j++) own[i][j] = d + j < hd ? x[d + j] + b[d + j] : 0.f;
+        }
+    const uint32_t pos = *a.pos, at = *a.slot;
     const float *cs = a.cos_t + (size_t)pos * (hd / 2), *sn = a.sin_t + (size_t)pos * (hd / 2);
     if (blockIdx.z == 2) {
         for (uint32_t i = 2 * threadIdx.x; i < a.n_rep * hd; i += 512) {
@@ -459,22 +481,20 @@ template <int NC> __global__ void __launch_bounds__(256) append_k(View v, Append
         return;
     }
     if (at >= v.max_len) return;
-    const bool key = blockIdx.z == 0;
-    const float *x = (key ? a.k : a.v) + head * hd, *b = (key ? a.bk : a.bv) + head * hd;
     const uint64_t base = (uint64_t)blockIdx.z * v.n_heads + head;
-    const uint32_t lo = at % kBlock, blk = at / kBlock;
-    const Tail tail = take_tail(v.tail_at + base * 4, blk, lo, lo + 1);
-    auto row = [&](uint32_t, uint32_t d, float *y) {
+    const uint32_t lo = at % kBlock;
+    Tail tail;
+    auto row = [&](uint32_t, int i, uint32_t d, float *y) {
 #pragma unroll
         for (uint32_t j = 0; j < 16; j += 2) {
-            const bool in = d + j < hd;                       // hd is even
-            const float x0 = in ? x[d + j] + b[d + j] : 0.f, x1 = in ? x[d + j + 1] + b[d + j + 1] : 0.f;
-            const float c = in && key ? cs[(d + j) / 2] : 1.f, s = in && key ? sn[(d + j) / 2] : 0.f;
-            y[j] = key ? x0 * c - x1 * s : x0;
-            y[j + 1] = key ? x0 * s + x1 * c : x1;
+            const bool turn = key && d + j < hd;              // hd is even
+            const float x0 = own[i][j], x1 = own[i][j + 1];
+            const float c = turn ? cs[(d + j) / 2] : 1.f, s = turn ? sn[(d + j) / 2] : 0.f;
+            y[j] = turn ? x0 * c - x1 * s : x0;
+            y[j + 1] = turn ? x0 * s + x1 * c : x1;
         }
     };
-    write_block<NC>(v, row, base, blk, lo, lo + 1, tail.slot, tail.held, lo + 1 < kBlock, key, maxes, red, stage);
+    write_block<NC, true>(v, row, base, at / kBlock, lo, lo + 1, tail, key, maxes, red, stage);
     put_tail(v.tail_at + base * 4, tail);
 }
 
