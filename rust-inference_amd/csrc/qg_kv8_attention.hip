@@ -537,18 +537,17 @@ __device__ __forceinline__ void take_q(const Problem &a, const Item &it, uint32_
     wave_sync();
 }
 
-template <uint32_t M> __device__ __forceinline__ void put_split(const Problem &a, uint32_t wg, const Item *it, uint32_t per)
+// cut: a workgroup's share begins inside `it`.  (Not a pointer to an item or none:
+// the item would have to lie in memory, and every use of it read it from there.)
+__device__ __forceinline__ void put_split(const Problem &a, uint32_t wg, bool cut, const Item &it, uint32_t per)
 {
     if (threadIdx.x) return;
     Split s{};
-    s.first = kNone;
-    if (it) {
-        s.first = it->start / per;
-        s.last = (it->start + it->t.chunks - 1) / per;
-        s.seq = it->seq;
-        s.head = it->head;
-        s.tile = it->tile;
-    }
+    s.first = cut ? it.start / per : kNone;
+    s.last = (it.start + it.t.chunks - 1) / per;
+    s.seq = it.seq;
+    s.head = it.head;
+    s.tile = it.tile;
     a.w.split[wg] = s;
 }
 
@@ -583,15 +582,15 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u, r = lane & 15u, g = lane >> 4;
     const uint32_t wg = place_of(blockIdx.x, gridDim.x);
     const Order order = order_of<kFewM>(a);
-    const uint32_t per = (order.total + gridDim.x - 1) / gridDim.x;
+    const uint32_t per = max((order.total + gridDim.x - 1) / gridDim.x, 1u);
     uint32_t at = wg * per;
     const uint32_t end = min(at + per, order.total);
     if (at >= end) {
-        put_split<kFewM>(a, wg, nullptr, per);
+        put_split(a, wg, false, Item{}, per);
         return;
     }
     Item it = find<kFewM>(a, at, order);
-    put_split<kFewM>(a, wg, at > it.start ? &it : nullptr, per);
+    put_split(a, wg, at > it.start, it, per);
     if (it.start >= end) return;                             // only its lead is here
     const uint64_t all = (uint64_t)a.v.n_seqs * a.v.n_heads;
     const uint8_t *kb, *vb;
@@ -783,15 +782,15 @@ template <int DP, int NP, int RT> __global__ void __launch_bounds__(256, 2) many
     float *const mine = (float *)(stage + wave * (kOne * 3 / 2));        // 16 rows of DP + 4 floats fit
     const uint32_t wg = place_of(blockIdx.x, gridDim.x);
     const Order order = order_of<M>(a);
-    const uint32_t per = (order.total + gridDim.x - 1) / gridDim.x;
+    const uint32_t per = max((order.total + gridDim.x - 1) / gridDim.x, 1u);
     uint32_t at = wg * per;
     const uint32_t end = min(at + per, order.total);
     if (at >= end) {
-        put_split<M>(a, wg, nullptr, per);
+        put_split(a, wg, false, Item{}, per);
         return;
     }
     Item it = find<M>(a, at, order);
-    put_split<M>(a, wg, at > it.start ? &it : nullptr, per);
+    put_split(a, wg, at > it.start, it, per);
     const uint64_t all = (uint64_t)a.v.n_seqs * a.v.n_heads;
     for (;;) {
         if (it.start >= end) break;                      // only its lead is here
