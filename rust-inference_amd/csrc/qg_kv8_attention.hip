@@ -566,11 +566,10 @@ __device__ __forceinline__ uint32_t place_of(uint32_t id, uint32_t n)
 // part's loads, which are requested before the join.
 //
 // Bound by the read of the cache where it is long: 64 sequences of up to 8192
-// tokens, 8 kv heads of 128, f16 rows 117 us (the 0.55 GB of codes at 4.7 TB/s; a
-// large copy does 5.0), one of 131072 tokens 47 (5.7 TB/s, half of it from the last
+// tokens, 8 kv heads of 128, f16 rows 107 us (the 0.55 GB of codes at 5.2 TB/s; a
+// large copy does 5.0), one of 131072 tokens 45 (6 TB/s, half of it from the last
 // level cache).  Short ones are a chain of latencies: lengths, codes, products,
-// join, about 11000 cycles at 49 tokens (6.1 us), 17400 at 2256 (10.6 with four
-// kv heads of 18 parts each).  Two workgroups a compute unit; three (with half
+// join, 5.9 us at 49 tokens, 9.5 at 2256 (four kv heads of 18 parts each).  Two workgroups a compute unit; three (with half
 // the registers) were slower, and so were parts of 8 or 16 blocks.
 constexpr uint32_t kFewM = 16;
 
@@ -765,9 +764,9 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
 //
 // Bound by the matrix cores and the vector units together (16 of the latter's
 // instructions a block and tile are exponentials): 1001 tokens of 32 heads of 128
-// in f32, two pieces of q and p, 43 us, 0.19 PFLOP/s of the formula and twice that
-// of products; 2048 new tokens of four sequences in f16 over 4096 positions each
-// 440 us, 0.70 PFLOP/s, where a large f16 matrix product does 1.11: matrix cores
+// in f32, two pieces of q and p, 41 us, 0.20 PFLOP/s of the formula and twice that
+// of products; up to 2048 new tokens of four sequences in f16 over 4096 positions
+// each 435 us, 0.71 PFLOP/s, where a large f16 matrix product does 1.11: matrix cores
 // busy in 31 % of the cycles, vector units in 42 %, waves waiting (data, barriers)
 // in 30 % of theirs.  Two workgroups of 48 KB a compute unit; larger tiles (256
 // pairs) spill: 744 against 480 us at that stage.  Rows that take 16-byte accesses
@@ -1168,9 +1167,10 @@ int launch_attention(const View &v, const Batch &b, uint32_t n_heads, const Rows
     // a block for each wave of few_k, two of many_k; more where the chunks
     // would not be counted in 31 bits (all tiles seeing the whole cache)
     a.chunk = kind == kFew ? 4u : 2u;
-    // measured (cycles): an item costs few_k 30000 and many_k 20000 whatever its
-    // length, a chunk 5500 and 4800; items of one length each need no balance
-    a.lead = kind == kFew && v.n_seqs == 1 ? 0u : 4u;
+    // what an item costs whatever its length, in chunks (us at 2, 3, 4, 6: 1001
+    // tokens of 32 heads 42.7, 41.2, 42.0, 45.0; 64 sequences' tokens 107, 108, 108, 111);
+    // single tokens of one sequence are items of one length and need no balance
+    a.lead = kind == kFew && v.n_seqs == 1 ? 0u : 3u;
     const uint64_t tiles = ((uint64_t)b.n_rows * a.n_rep + tile_rows(kind) - 1) / tile_rows(kind) + v.n_seqs;
     while (tiles * v.n_heads * (v.n_blocks / a.chunk + 1 + a.lead) >> 31) a.chunk *= 2;
     a.w = work_at(work, workgroups(n_cu), tile_rows(kind));
