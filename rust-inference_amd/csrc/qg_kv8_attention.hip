@@ -35,6 +35,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace qg8 {
 namespace {
@@ -1021,8 +1022,11 @@ template <int DP, int NP, int RT> __global__ void __launch_bounds__(256, 2) many
 // in slot 1, the others' in slot 0).  Grid: (workgroups - 1, row groups); the
 // workgroup of the second part does it.  DP / 4 lanes take a row's elements; few
 // rows of many parts (PARTS): the other threads take parts in turn; else they
-// take rows.  Bound by its launch and two dependent reads: 4 us behind few_k, 6.8
-// and 14 behind many_k's tiles of 64 and 128 pairs (up to 67 MB of parts).
+// take rows.  Bound by its launch and a few dependent reads where there are few
+// parts: 4 to 5.5 us behind few_k, 7.6 and 14 behind many_k's tiles of 64 and 128
+// pairs (up to 67 MB of parts).  A short prompt over a long cache has many parts a
+// tile: 32 of them 8.6 us with eight on their way together and eight row groups (25.8
+// one after the other, 13.0 with four groups).
 template <uint32_t M, int DP, bool PARTS> __global__ void __launch_bounds__(256) merge_k(Problem a)
 {
     constexpr uint32_t L = DP / 4, N = 256 / L;            // 192 / 4 = 48: 5 groups, 16 lanes idle
@@ -1041,12 +1045,28 @@ template <uint32_t M, int DP, bool PARTS> __global__ void __launch_bounds__(256)
             l = l * e + k * f;
             x.x = x.x * e + o.x * f; x.y = x.y * e + o.y * f; x.z = x.z * e + o.z * f; x.w = x.w * e + o.w * f;
         };
-        if (grp < N)
-            for (uint32_t w = s.first + (PARTS ? grp : 0); w <= s.last; w += PARTS ? N : 1) {
-                const uint64_t at = ((uint64_t)w * 2 + (w == s.first ? 1u : 0u)) * M + r;
-                const float2 t = *(const float2 *)(a.w.ml + at * 2);
-                add(t.x, t.y, *(const float4 *)(a.w.part + at * DP + d));
+        // the thread's parts, AT of them on their way together
+        auto take = [&](auto at_once) {
+            constexpr uint32_t AT = decltype(at_once)::value, step = PARTS ? N : 1;
+            for (uint32_t w0 = s.first + (PARTS ? grp : 0); w0 <= s.last; w0 += AT * step) {
+                float2 t[AT];
+                float4 o[AT];
+#pragma unroll
+                for (uint32_t j = 0; j < AT; j++) {              // the last one again behind it
+                    const uint32_t w = min(w0 + j * step, s.last);
+                    const uint64_t at = ((uint64_t)w * 2 + (w == s.first ? 1u : 0u)) * M + r;
+                    t[j] = *(const float2 *)(a.w.ml + at * 2);
+                    o[j] = *(const float4 *)(a.w.part + at * DP + d);
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < AT; j++)
+                    if (w0 + j * step <= s.last) add(t[j].x, t[j].y, o[j]);
             }
+        };
+        if (grp < N) {
+            if (s.last - s.first < 2 * (PARTS ? N : 1)) take(std::integral_constant<uint32_t, 2>{});
+            else take(std::integral_constant<uint32_t, 8>{});
+        }
         if (PARTS) {
             if (grp < N) {
                 if (lane == 0) { sm[grp] = m; sl[grp] = l; }
@@ -1093,11 +1113,14 @@ enum Kind { kFew, kMany64, kMany128 };
 Kind kind_of(const View &v, uint64_t n_rows, bool starts, uint64_t n_rep, int n_cu)
 {
     const uint64_t pairs = starts ? n_rows * n_rep / std::min<uint64_t>(v.n_seqs, n_rows ? n_rows : 1) : n_rep;
+    // two tiles of 16 rather than half of one of 64 (us: 24 pairs over 8000 positions
+    // 21 against 54, 32 of eight sequences 33 against 43; 56 of 16 sequences 72
+    // against 62)
     if (pairs <= 32) return kFew;
     // tiles of 128 pairs where there are enough of them for the workgroups: with
     // fewer, the items are cut anyway, and the smaller ones have less to begin and
-    // end with (1001 tokens of 32 heads 44.6 against 54.4 us, f32; 5000 of them over
-    // four sequences 597 against 452, f16)
+    // end with (1001 tokens of 32 heads 41 against 47 us, f32; 5200 of them over four
+    // sequences 610 against 459, f16)
     const uint64_t tiles = (n_rows * n_rep + 127) / 128 * v.n_heads;
     return pairs <= 64 || v.dp > 128 || tiles < workgroups(n_cu) ? kMany64 : kMany128;
 }
@@ -1113,7 +1136,7 @@ template <int DP, int NP, int RT> int launch_many(Problem &a, uint32_t wgs, hipS
     hipLaunchKernelGGL((many_k<DP, NP, RT>), dim3(wgs), dim3(256), lds, st, a);
     if (hipPeekAtLastError() != hipSuccess) return -1;
     if (a.v.n_blocks > a.chunk)
-        hipLaunchKernelGGL((merge_k<64 * RT, DP, false>), dim3(wgs - 1, 4), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((merge_k<64 * RT, DP, false>), dim3(wgs - 1, 8), dim3(256), 0, st, a);
     return hipPeekAtLastError() == hipSuccess ? 0 : -1;
 }
 
