@@ -110,10 +110,10 @@ int qg_kv8_read_dev(qg_ctx *ctx, const qg_kv8 *kv, size_t seq, size_t n_seqs, si
  * no position to see (one below 0) gives zeros; a row at a position past max_len
  * sees the positions there are.  n_heads at most 65535, n_rows * n_heads below
  * 2^31 (QG_ERR_SHAPE).  q and out have one type; f32 rows are computed to f32
- * precision (two f16 pieces of q and of p), f16 rows with f16 p, sums in f32.  d_work: qg_kv8_attention_work
- * bytes of device memory (16-byte aligned) that no other call in flight uses
- * (captured graphs that may run side by side need one each); its contents need
- * not be kept.  QG_ERR_SHAPE when work_bytes is less. */
+ * precision (two f16 pieces of q and of p), f16 rows with f16 p, sums in f32.
+ * d_work: qg_kv8_attention_work bytes of device memory (16-byte aligned) that no
+ * other call in flight uses (captured graphs that may run side by side need one
+ * each); its contents need not be kept.  QG_ERR_SHAPE when work_bytes is less. */
 int qg_kv8_attention_dev(qg_ctx *ctx, const qg_kv8 *kv, const qg_batch *batch, size_t n_heads, const qg_rows *q,
                          float scale, size_t window, const qg_rows *out, void *d_work, size_t work_bytes,
                          void *stream);

@@ -403,9 +403,9 @@ __device__ void write_whole(const View &v, const Rows &x, uint64_t row_at, uint6
 }
 
 // Grid: (items, heads, keys / values).  Bound by the latency of a few dependent
-// loads where there is little (one token 4.2 us, 1001 tokens of 8 heads of 128 in
-// f32 7.7), by the memory and its latency where there is much (32 prompts of up to
-// 2048 tokens, 8 heads of 128 in f16, 194 MB: 54 us, 3.6 TB/s).
+// loads where there is little (one token 3.6 us, 1001 tokens of 8 heads of 128 in
+// f32 7.5), by the memory and its latency where there is much (32 prompts of up to
+// 2048 tokens, 8 heads of 128 in f16, 194 MB: 53 us, 3.7 TB/s).
 //
 // The scale of a block follows from its largest magnitude, so a new token in a
 // block that is partly there costs its own row and 32 remembered magnitudes
@@ -452,7 +452,8 @@ __global__ void __launch_bounds__(256, NC == 1 ? 5 : 2) write_k(View v, Batch b,
 // A decode step's projections of one token (Append): q and k with their biases
 // rotated, v with its own, k and v written as the token's place of a cache of one
 // sequence.  Grid: (1, kv heads, keys / values / the kv head's query heads).
-// One launch for what was two (qkv rotation, write_k), each a few dependent loads.
+// One launch for what was two (the rotation, then write_k), each a chain of dependent
+// loads: 5 to 6 us inside a decode step.
 template <int NC> __global__ void __launch_bounds__(256) append_k(View v, Append a)
 {
     __shared__ uint32_t maxes[kBlock], red[4];

@@ -767,9 +767,9 @@ template <int DP, int NP> __global__ void __launch_bounds__(256, DP <= 128 ? 2 :
 // instructions a block and tile are exponentials): 1001 tokens of 32 heads of 128
 // in f32, two pieces of q and p, 41 us, 0.20 PFLOP/s of the formula and twice that
 // of products; up to 2048 new tokens of four sequences in f16 over 4096 positions
-// each 435 us, 0.71 PFLOP/s, where a large f16 matrix product does 1.11: matrix cores
-// busy in 31 % of the cycles, vector units in 42 %, waves waiting (data, barriers)
-// in 30 % of theirs.  Two workgroups of 48 KB a compute unit; larger tiles (256
+// each 406 us with the merge, 0.76 PFLOP/s, where a large f16 matrix product does
+// 1.11: matrix cores busy in 33 % of the cycles, vector units in 56 %, waves waiting
+// (data, barriers) in 27 % of theirs.  Two workgroups of 48 KB a compute unit; larger tiles (256
 // pairs) spill: 744 against 480 us at that stage.  Rows that take 16-byte accesses
 // go straight from and to memory; through LDS they cost a part 10000 cycles more.
 template <int DP, int NP, int RT> __global__ void __launch_bounds__(256, 2) many_k(Problem a)
