@@ -14,7 +14,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from test_kv8_gpu import NP, all_quantised, dev, i32, rows, write
+from test_kv8_gpu import NP, all_quantised, dev, i32, read, rows, write
 
 pytestmark = pytest.mark.gpu
 
@@ -351,6 +351,82 @@ def test_write_then_attend(rinf, ctx):
         for s in range(2):
             want, tol = reference(q[starts[s]:starts[s + 1]], all_quantised(hk[s]), all_quantised(hv[s]), lens[s] - n[s], 0, hd ** -0.5)
             compare(out.cpu().numpy()[starts[s]:starts[s + 1]], want, tol, False)
+    cache.free()
+
+
+@pytest.mark.parametrize("rows_each", [1, 45])
+def test_captured_step_of_a_batch(rinf, ctx, rows_each):
+    """Write, attention and log probabilities as one captured step of a batch; between the replays the
+    lengths, the split of the rows and the tokens change, and eager calls run on the same cache."""
+    import torch
+    rng = np.random.default_rng(23 + rows_each)
+    kv, hd, heads, seqs, most = 2, 64, 4, 3, 400
+    n = rows_each * seqs
+    cache = ctx.kv8(seqs, kv, hd, most)
+    f32, dev0 = torch.float32, "cuda"
+    k, v = torch.zeros(n, kv, hd, device=dev0), torch.zeros(n, kv, hd, device=dev0)
+    q, out = torch.zeros(n, heads, hd, device=dev0), torch.zeros(n, heads, hd, device=dev0)
+    lens, starts = i32([0] * seqs), i32([0] * (seqs + 1))
+    ids = torch.zeros(n, 1, dtype=torch.int32, device=dev0)
+    lp, ent, tids, tlp = (torch.zeros(n, c, dtype=d, device=dev0) for c, d in ((1, f32), (1, f32), (5, torch.int32), (5, f32)))
+    work = torch.zeros(max(16, cache.attention_work(n, heads)), dtype=torch.uint8, device=dev0)
+    lwork = torch.zeros(max(16, ctx.logprobs_work(n, heads * hd, 5)), dtype=torch.uint8, device=dev0)
+    torch.cuda.synchronize()
+
+    def step(stream):
+        cache.write_dev(k, v, lens, starts, stream=stream)
+        cache.attention_dev(q, out, lens, work, starts, stream=stream)
+        ctx.logprobs_dev(out.view(n, heads * hd), ids, lp, ent, tids, tlp, lwork, stream=stream)
+
+    st, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        step(torch.cuda.current_stream().cuda_stream)
+    hk, hv = ([np.zeros((0, kv, hd), np.float32)] * seqs for _ in range(2))
+    for turn in range(5):
+        m = [rows_each] * seqs if rows_each == 1 else [int(x) for x in rng.multinomial(n - turn, [0.5, 0.1, 0.4])]
+        nk, nv = ([rows(rng, x, kv, hd) for x in m] for _ in range(2))
+        hk, hv = ([np.concatenate([a, b]) for a, b in zip(h, x)] for h, x in ((hk, nk), (hv, nv)))
+        total, at = [len(h) for h in hk], np.concatenate([[0], np.cumsum(m)])
+        hq, given = rng.standard_normal((n, heads, hd)).astype(np.float32), rng.integers(0, heads * hd, (n, 1))
+        k[:at[-1]].copy_(dev(np.concatenate(nk))), v[:at[-1]].copy_(dev(np.concatenate(nv))), q.copy_(dev(hq))
+        lens.copy_(i32(total)), starts.copy_(i32(at)), ids.copy_(i32(given)), out.fill_(7.0)
+        torch.cuda.synchronize()
+        g.replay() if turn % 2 == 0 else step(st.cuda_stream)
+        torch.cuda.synchronize()
+        got = out.cpu().numpy()
+        assert (got[at[-1]:] == 7.0).all()
+        for s in range(seqs):
+            want, tol = reference(hq[at[s]:at[s + 1]], all_quantised(hk[s]), all_quantised(hv[s]), total[s] - m[s], 0, hd ** -0.5)
+            compare(got[at[s]:at[s + 1]], want, tol, False)
+        x = got.reshape(n, heads * hd).astype(np.float64)
+        p = x - x.max(1, keepdims=True)
+        p -= np.log(np.exp(p).sum(1, keepdims=True))
+        # 256 terms: sums and exponents within 300 steps of 2^-24
+        assert np.abs(lp.cpu().numpy() - np.take_along_axis(p, given, 1)).max() < 300 * U * np.abs(p).max()
+        order = np.argsort(-x, axis=1, kind="stable")[:, :5]
+        assert (tids.cpu().numpy() == order).all()
+    cache.free()
+
+
+def test_offsets_past_32_bits(rinf, ctx):
+    """The end of a cache whose codes lie past 4 GB, by single rows and by many."""
+    rng = np.random.default_rng(29)
+    kv, hd, heads, most, n = 4, 256, 8, 1 << 20, 40
+    cache = ctx.kv8(3, kv, hd, most)
+    assert cache.nbytes > 6 << 30
+    k, v = rows(rng, n, kv, hd), rows(rng, n, kv, hd)
+    none = np.zeros((0, kv, hd), np.float32)
+    write(ctx, cache, [none, none, k], [none, none, v], [0, 0, most])
+    zeros = np.zeros((24, kv, hd), np.float32)                # the 24 positions of its block before them
+    kq, vq = all_quantised(np.concatenate([zeros, k])), all_quantised(np.concatenate([zeros, v]))
+    gk, gv = read(ctx, cache, 2, most - 64, 64)
+    np.testing.assert_array_equal(gk, kq)
+    np.testing.assert_array_equal(gv, vq)
+    for m in (1, n):
+        q = rng.standard_normal((m, heads, hd)).astype(np.float32)
+        got = run(ctx, cache, q, [0, 0, most], [0, 0, 0, m], window=24)
+        want, tol = reference(q, kq, vq, 64 - m, 24, hd ** -0.5)
+        compare(got, want, tol, False)
     cache.free()
 
 
