@@ -311,7 +311,8 @@ template <bool F16, bool TOP> __global__ void __launch_bounds__(kThreads) final_
 }
 
 // Parts of a row: enough for about two workgroups per compute unit, of 2048
-// elements at least.
+// elements at least (64 rows of 128256 with 20 alternatives 19.8 us; three and four
+// a compute unit 29 and 23).
 uint32_t parts_of(size_t n_rows, size_t n_cols, int n_cu)
 {
     const size_t want = 2u * (size_t)(n_cu > 0 ? n_cu : 256) / (n_rows ? n_rows : 1), most = (n_cols + 2047) / 2048;
